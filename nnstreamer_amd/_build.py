@@ -81,7 +81,9 @@ def write_ninja(debug: bool = False) -> str:
     py_inc = sysconfig.get_paths()["include"]
     opt = "-O0 -g" if debug else "-O3"
     common = f"{opt} -fPIC -std=c++17 -Wall -Wno-unused-function -Wno-unused-variable -Wno-sign-compare -I{CSRC} -I{ROOT}/include -D_GLIBCXX_USE_CXX11_ABI=1"
-    hip_flags = f"-x hip --offload-arch={ARCH} -munsafe-fp-atomics -ffp-contract=fast"
+    # no packed fp32 instructions: some of their forms have given wrong results on this hardware now and then
+    hip_flags = (f"-x hip --offload-arch={ARCH} -munsafe-fp-atomics -ffp-contract=fast "
+                 "-Xclang -target-feature -Xclang -packed-fp32-ops")
     torch_flags = " ".join(f"-isystem {p}" for p in tinc) + " -D__HIP_PLATFORM_AMD__=1 -DUSE_ROCM=1 -Wno-deprecated-declarations -Wno-unknown-pragmas"
     py_flags = f"-isystem {pybind11.get_include()} -isystem {py_inc} -fvisibility=hidden"
     lib_dirs = " ".join(f"-L{p} -Wl,-rpath,{p}" for p in tlib)
