@@ -1,0 +1,666 @@
+// Attention of new tokens over a paged key/value cache, gfx950.
+//
+//   o_i = sum_j softmax_j(scale * q_i . k_j) v_j   over the keys j that row i sees
+//
+// Rows: the new tokens of one sequence times the query heads that share one
+// key/value head, packed token-major (row = token * group + head in group), so
+// a key is fetched once for the whole group.  Both products run transposed on
+// 32 x 32 matrix instructions,
+//
+//   S^T = K Q^T   (A = 32 keys, B = 32 rows)    O^T = V^T P^T   (A = V^T, B = P^T),
+//
+// so that a lane holds one row's scores: 16 of a block's 32 keys, the lane 32
+// further the other 16.  The running maximum and sum of the softmax are then
+// one exchange between two lanes per block, the rescale of O^T is one factor
+// per lane, and P^T is already where the second product wants it -- the order
+// of the summed index is free as long as V^T uses the same one (slot j of lane
+// half h = key 16 s + 8 (j / 4) + 4 h + j % 4).  Scores, maxima, sums and O are
+// fp32; P is rounded to the cache's type for the second product (weights in
+// [0, 1], relative error half a step, as the output's own rounding).
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "kernels/attn.h"
+
+namespace nnsx {
+namespace kernels {
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int kRows = 32;   // rows of one item
+constexpr int kKeys = 32;   // keys of one block
+constexpr int kCus = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNegInf = -__builtin_huge_valf();
+
+struct BF16 {};
+struct F16 {};
+struct F32 {};
+
+// 8 slots of the summed index for one lane: 16-bit types
+template <typename T>
+__device__ __forceinline__ f32x16 mfma16(u32x4 a, u32x4 b, f32x16 c);
+template <>
+__device__ __forceinline__ f32x16 mfma16<BF16>(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x16 mfma16<F16>(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<BF16>(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<F16>(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
+}
+// exponent all ones in either half
+template <typename T>
+__device__ __forceinline__ bool nonfinite2(uint32_t x);
+template <>
+__device__ __forceinline__ bool nonfinite2<BF16>(uint32_t x) {
+  return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+}
+template <>
+__device__ __forceinline__ bool nonfinite2<F16>(uint32_t x) {
+  return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u;
+}
+
+// the other half's value of the same row
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+
+// ------------------------------------------------------------------- plan ----
+// Work is cut into items: (sequence, tile of rows, split of its key blocks).
+// Lengths live on the device, so every workgroup derives its own item from
+// them: the key blocks of all (sequence, tile) pairs are summed, a split is
+// chosen so long that about `target` items result (more only because every
+// pair has at least one), and the item's pair is found by a running sum over
+// the sequences.  target = 0: no split.
+struct Item {
+  int b;        // sequence; -1: nothing to do.  B: the rows behind the last sequence
+  int tile, split, splits, slot;
+  int chunk;    // key blocks of a split
+  int n, t0;    // new tokens, first token row
+  int len, keys;  // length; keys that the table can hold of them
+};
+
+struct Seq {
+  int n, t0, len, keys, tiles, blocks;
+};
+
+template <int ROWS, int KEYS>
+__device__ __forceinline__ Seq seq_of(const PagedAttnArgs& a, int b) {
+  Seq s;
+  const int T = a.p.T;
+  auto at = [&](int i) { return i == 0 ? 0 : min(max(a.p.cu[i], 0), T); };
+  s.t0 = at(b);
+  const int t1 = b < a.p.B ? at(b + 1) : T;
+  s.n = max(t1 - s.t0, 0);
+  s.len = b < a.p.B ? max(a.p.len[b], 0) : 0;
+  s.keys = static_cast<int>(min(static_cast<int64_t>(s.len), static_cast<int64_t>(a.p.width) * a.p.page));
+  s.tiles = static_cast<int>((static_cast<int64_t>(s.n) * a.group + ROWS - 1) / ROWS);
+  const int64_t first = static_cast<int64_t>(s.len) - s.n - a.window + 1;  // first key the first token sees
+  const int lo = a.window > 0 ? static_cast<int>(min(max(first, static_cast<int64_t>(0)), static_cast<int64_t>(s.keys))) : 0;
+  s.blocks = s.n > 0 ? (s.keys + KEYS - 1) / KEYS - lo / KEYS : 0;
+  return s;
+}
+
+// value and running sum over the workgroup (wave shuffles, then the waves' sums)
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t* total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int64_t x = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  __syncthreads();
+  if (lane == 63) sh[w] = x;
+  __syncthreads();
+  int64_t base = 0, sum = 0;
+  for (int i = 0; i < static_cast<int>(blockDim.x >> 6); ++i) {
+    if (i < w) base += sh[i];
+    sum += sh[i];
+  }
+  *total = sum;
+  return base + x - v;  // exclusive
+}
+
+// PAIRS false: `index` counts items; PAIRS true: (sequence, tile) pairs, and
+// the item's slot is that of the pair's first split
+template <int ROWS, int KEYS, bool PAIRS>
+__device__ Item find_item(const PagedAttnArgs& a, int index, int64_t* sh /* [kWaves] */, int* found /* [5] */) {
+  Item it;
+  const int tid = threadIdx.x, nt = blockDim.x, B1 = a.p.B + 1;
+  int chunk = 1 << 28;
+  if (a.target > 0) {
+    int64_t w = 0, total;
+    for (int b = tid; b < B1; b += nt) {
+      const Seq s = seq_of<ROWS, KEYS>(a, b);
+      w += static_cast<int64_t>(s.tiles) * s.blocks;
+    }
+    block_scan(w, sh, &total);
+    const int64_t c = (total + a.target - 1) / a.target;
+    chunk = static_cast<int>(min(max(c, static_cast<int64_t>(a.min_chunk)), static_cast<int64_t>(1 << 28)));
+  }
+  if (tid == 0) found[0] = -1;
+  int64_t carry = 0;  // pairs << 32 | items
+  for (int b0 = 0; b0 < B1; b0 += nt) {
+    const int b = b0 + tid;
+    int64_t mine = 0;
+    int tiles = 0, splits = 1;
+    if (b < B1) {
+      const Seq s = seq_of<ROWS, KEYS>(a, b);
+      tiles = s.tiles;
+      splits = max((s.blocks + chunk - 1) / chunk, 1);
+      mine = (static_cast<int64_t>(tiles) << 32) + static_cast<int64_t>(tiles) * splits;
+    }
+    int64_t total;
+    const int64_t first = carry + block_scan(mine, sh, &total);
+    const int first_item = static_cast<int>(first & 0xffffffff), first_pair = static_cast<int>(first >> 32);
+    const int rel = index - (PAIRS ? first_pair : first_item);
+    if (rel >= 0 && rel < (PAIRS ? tiles : tiles * splits)) {
+      const int tile = PAIRS ? rel : rel / splits;
+      found[0] = b;
+      found[1] = tiles - 1 - tile;  // the tiles with the most keys first: the short ones fill the tail
+      found[2] = PAIRS ? 0 : rel % splits;
+      found[3] = splits;
+      found[4] = first_item + tile * splits + found[2];
+    }
+    carry += total;
+    if (index < (PAIRS ? carry >> 32 : carry & 0xffffffff)) break;  // (the same in every thread)
+  }
+  __syncthreads();
+  it.b = __builtin_amdgcn_readfirstlane(found[0]);
+  if (it.b < 0) return it;
+  it.tile = __builtin_amdgcn_readfirstlane(found[1]);
+  it.split = __builtin_amdgcn_readfirstlane(found[2]);
+  it.splits = __builtin_amdgcn_readfirstlane(found[3]);
+  it.slot = __builtin_amdgcn_readfirstlane(found[4]);
+  it.chunk = __builtin_amdgcn_readfirstlane(chunk);
+  const Seq s = seq_of<ROWS, KEYS>(a, it.b);
+  it.n = __builtin_amdgcn_readfirstlane(s.n);
+  it.t0 = __builtin_amdgcn_readfirstlane(s.t0);
+  it.len = __builtin_amdgcn_readfirstlane(s.len);
+  it.keys = __builtin_amdgcn_readfirstlane(s.keys);
+  return it;
+}
+
+// keys [lo, hi) that the tokens i0 .. i1 of an item see
+__device__ __forceinline__ void key_range(const PagedAttnArgs& a, const Item& it, int i0, int i1, int* lo, int* hi) {
+  const int64_t first = static_cast<int64_t>(it.len) - it.n;
+  *hi = a.causal ? static_cast<int>(min(max(first + i1 + 1, static_cast<int64_t>(0)), static_cast<int64_t>(it.keys)))
+                 : it.keys;
+  *lo = a.window > 0 ? static_cast<int>(min(max(first + i0 - a.window + 1, static_cast<int64_t>(0)),
+                                            static_cast<int64_t>(it.keys)))
+                     : 0;
+  if (*hi < *lo) *hi = *lo;
+}
+
+// workspace of a split call: per (item slot, kv head) kRows x (d floats) and kRows x (max, sum)
+__host__ __device__ __forceinline__ size_t part_floats(int rows, int d) { return static_cast<size_t>(rows) * (d + 2); }
+
+// ------------------------------------------------------------ stream kernel ----
+// One workgroup per item of 32 rows; its four waves take key blocks in turn,
+// each on its own (no barrier in the loop) and straight from global memory into
+// the matrix instructions' registers: a lane loads 16 bytes of a key for S^T;
+// for O^T the lanes of a half load a whole row of V (DP / 32 neighbouring
+// columns each, so column = (DP / 32) * row of the tile + tile) and eight rows'
+// halves are interleaved with byte permutes.  Four partial (max, sum, O) are
+// joined through LDS at the end.
+template <typename T>
+struct Elem { using type = uint16_t; static constexpr bool wide = false; };
+template <>
+struct Elem<F32> { using type = float; static constexpr bool wide = true; };
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) void paged_attn_stream(PagedAttnArgs a) {
+  using E = typename Elem<T>::type;
+  constexpr bool WIDE = Elem<T>::wide;
+  constexpr int NB = DP / 32;            // 32-column tiles of O^T
+  constexpr int KC = WIDE ? DP / 8 : DP / 16;  // 16-byte pieces of a key per lane
+  constexpr int PIECE = WIDE ? 4 : 8;    // elements of a piece
+  __shared__ int64_t sh_scan[kWaves];
+  __shared__ int sh_found[5];
+  __shared__ float sh_ml[kWaves][2][kRows];
+  __shared__ float sh_o[2][NB * 16][64];
+
+  const int head = static_cast<int>(blockIdx.x % a.hkv);
+  const int slot = static_cast<int>(blockIdx.x / a.hkv);
+  const Item it = find_item<kRows, kKeys, false>(a, slot, sh_scan, sh_found);
+  if (it.b < 0) return;
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int rows = it.n * a.group;  // (fits: T * hq < 2^31)
+  const int row = it.tile * kRows + col;
+  const bool live = row < rows;
+  const int tok = row / a.group, gh = row - tok * a.group;
+  // what this lane's row sees
+  int rlo, rhi, tlo, thi;
+  key_range(a, it, tok, tok, &rlo, &rhi);
+  if (!live) rhi = rlo = 0;
+  {
+    const int i0 = it.tile * kRows / a.group, i1 = min((it.tile * kRows + kRows - 1) / a.group, it.n - 1);
+    key_range(a, it, i0, i1, &tlo, &thi);
+  }
+  int blk0 = tlo / kKeys, blk1 = (thi + kKeys - 1) / kKeys;
+  {  // this split's blocks
+    const int64_t s0 = blk0 + static_cast<int64_t>(it.split) * it.chunk;
+    const int64_t s1 = s0 + it.chunk;
+    blk0 = static_cast<int>(min(s0, static_cast<int64_t>(blk1)));
+    blk1 = static_cast<int>(min(s1, static_cast<int64_t>(blk1)));
+  }
+
+  const E* qp = static_cast<const E*>(a.q) + static_cast<int64_t>(it.t0 + tok) * a.qt +
+                static_cast<int64_t>(head * a.group + gh) * a.qh;
+  const E* kbase = static_cast<const E*>(a.k) + head * a.kh;
+  const E* vbase = static_cast<const E*>(a.v) + head * a.vh;
+  const int* table = a.p.table + static_cast<int64_t>(it.b) * a.p.tstride;
+
+  u32x4 q[KC];
+#pragma unroll
+  for (int s = 0; s < KC; ++s) {
+    const int d = (2 * s + half) * PIECE;
+    q[s] = (u32x4)(0u);
+    if (live && d < a.d) q[s] = *reinterpret_cast<const u32x4*>(qp + d);
+  }
+
+  f32x16 o[NB];
+#pragma unroll
+  for (int m = 0; m < NB; ++m) o[m] = (f32x16)(0.f);
+  float mx = kNegInf, sum = 0.f;
+  const float c = a.scale * kLog2e;
+
+  u32x4 k[KC];
+  // V: 16 rows a lane half, NB neighbouring columns: NB / 2 words (16 bit) or NB (32 bit)
+  constexpr int VW = WIDE ? NB : NB / 2;
+  uint32_t v[16][VW];
+  const int vcol = NB * col;
+
+  // page of this lane's key (lane & 31) in block blk; -1: not there
+  auto page_of = [&](int blk) {
+    const int key = blk * kKeys + col;
+    int id = -1;
+    if (key < it.keys) {
+      id = table[key / a.p.page];
+      if (id < 0 || id >= a.p.pages) id = -1;
+    }
+    return id;
+  };
+  auto load_k = [&](int blk, int id) {
+    const int key = blk * kKeys + col;
+    const E* p = kbase + static_cast<int64_t>(id) * a.kp + static_cast<int64_t>(key % a.p.page) * a.kr;
+#pragma unroll
+    for (int s = 0; s < KC; ++s) {
+      const int d = (2 * s + half) * PIECE;
+      k[s] = (u32x4)(0u);
+      if (id >= 0 && d < a.d) k[s] = *reinterpret_cast<const u32x4*>(p + d);
+    }
+  };
+  auto load_v = [&](int blk, int id) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int kk = 8 * (i / 4) + 4 * half + i % 4;
+      const int kid = __shfl(id, kk);
+      const int key = blk * kKeys + kk;
+      const E* p = vbase + static_cast<int64_t>(kid) * a.vp + static_cast<int64_t>(key % a.p.page) * a.vr + vcol;
+#pragma unroll
+      for (int w = 0; w < VW; ++w) v[i][w] = 0u;
+      if (kid >= 0 && vcol < a.d) {
+        if constexpr (VW == 1) {
+          v[i][0] = *reinterpret_cast<const uint32_t*>(p);
+        } else if constexpr (VW == 2) {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+          v[i][0] = x[0];
+          v[i][1] = x[1];
+        } else {
+#pragma unroll
+          for (int w = 0; w < VW; w += 4) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(p + w * (WIDE ? 1 : 2));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i][w + e] = x[e];
+          }
+        }
+      }
+    }
+  };
+
+  int blk = blk0 + wave;
+  int id = blk < blk1 ? page_of(blk) : -1;
+  if (blk < blk1) {
+    load_k(blk, id);
+    load_v(blk, id);
+  }
+  int idn = blk + kWaves < blk1 ? page_of(blk + kWaves) : -1;
+  while (blk < blk1) {
+    const int next = blk + kWaves;
+    const int key0 = blk * kKeys;
+    const uint32_t there = static_cast<uint32_t>(__ballot(id >= 0));  // (lanes 0 .. 31: the block's keys)
+    f32x16 s = (f32x16)(0.f);
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int i = 0; i < KC; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k[i][e]), __uint_as_float(q[i][e]), s, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < KC; ++i) s = mfma16<T>(k[i], q[i], s);
+    }
+    if (next < blk1) load_k(next, idn);
+    // every row of the tile sees every key of the block?
+    const bool full = there == 0xffffffffu && __all(!live || (rlo <= key0 && key0 + kKeys <= rhi));
+    if (!full) {
+      const int lo = rlo - key0 - 4 * half, hi = rhi - key0 - 4 * half;
+      const uint32_t bits = there >> (4 * half);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int kk = 8 * (i / 4) + i % 4;
+        if (!(kk >= lo && kk < hi && (bits >> kk & 1))) s[i] = kNegInf;
+      }
+    }
+    float bm = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) bm = fmaxf(bm, s[i]);
+    bm = fmaxf(bm, other_half(bm));
+    const float nm = fmaxf(mx, bm * c);
+    const float base = nm == kNegInf ? 0.f : nm;  // (a row that has seen nothing yet)
+    if (__any(nm > mx)) {
+      const float f = __builtin_amdgcn_exp2f(mx - base);
+      sum *= f;
+#pragma unroll
+      for (int m = 0; m < NB; ++m)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[m][i] *= f;
+      mx = nm;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = __builtin_amdgcn_exp2f(s[i] * c - base);
+      sum += s[i];
+    }
+
+    // O^T += V^T P^T.  Where a key is hidden from some rows only, its weight
+    // is 0 there, but 0 times an infinite or NaN value is not: such a block is
+    // added key by key, and only to the rows that see the key.
+    bool odd = false;
+    if (!full) {
+      bool nf = false;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+          if constexpr (WIDE)
+            nf |= (v[i][w] & 0x7f800000u) == 0x7f800000u;
+          else
+            nf |= nonfinite2<T>(v[i][w]);
+        }
+      odd = __any(nf);
+    }
+    if constexpr (WIDE) {
+      if (!odd) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+          for (int m = 0; m < NB; ++m)
+            o[m] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(v[i][m]), s[i], o[m], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            const int key = key0 + 8 * (i / 4) + 4 * h + i % 4;
+            const bool sees = key >= rlo && key < rhi && (there >> (key - key0) & 1);
+            const float p = half == h ? s[i] : 0.f;
+#pragma unroll
+            for (int m = 0; m < NB; ++m) {
+              const float x = half == h ? __uint_as_float(v[i][m]) : 0.f;
+              const f32x16 t = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p, (f32x16)(0.f), 0, 0, 0);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[m][e] = sees ? o[m][e] + t[e] : o[m][e];
+            }
+          }
+      }
+    } else {
+      u32x4 p[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[t][e] = pack2<T>(s[8 * t + 2 * e], s[8 * t + 2 * e + 1]);
+#pragma unroll
+      for (int m = 0; m < NB; ++m) {
+        u32x4 vt[2];
+        constexpr uint32_t kLow = 0x05040100u, kHigh = 0x07060302u;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            vt[t][e] = __builtin_amdgcn_perm(v[8 * t + 2 * e + 1][m / 2], v[8 * t + 2 * e][m / 2], m % 2 ? kHigh : kLow);
+        if (!odd) {
+          o[m] = mfma16<T>(vt[0], p[0], o[m]);
+          o[m] = mfma16<T>(vt[1], p[1], o[m]);
+        } else {
+#pragma unroll 1
+          for (int kk = 0; kk < kKeys; ++kk) {
+            const int key = key0 + kk;
+            const bool sees = key >= rlo && key < rhi && (there >> kk & 1);
+            const int i = 4 * (kk / 8) + kk % 4;
+            const uint32_t pick = half == (kk >> 2 & 1) ? (i & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
+            f32x16 t = (f32x16)(0.f);
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              u32x4 va, pa;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t mask = i / 2 == 4 * g + e ? pick : 0u;
+                va[e] = vt[g][e] & mask;
+                pa[e] = p[g][e] & mask;
+              }
+              t = mfma16<T>(va, pa, t);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[m][e] = sees ? o[m][e] + t[e] : o[m][e];
+          }
+        }
+      }
+    }
+    if (next < blk1) load_v(next, idn);
+    id = idn;
+    idn = next + kWaves < blk1 ? page_of(next + kWaves) : -1;
+    blk = next;
+  }
+  sum += other_half(sum);
+
+  // join the waves: a common maximum, then O in two rounds (2, 3 -> 0, 1; 1 -> 0)
+  if (half == 0) {
+    sh_ml[wave][0][col] = mx;
+    sh_ml[wave][1][col] = sum;
+  }
+  __syncthreads();
+  float M = kNegInf, L = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) M = fmaxf(M, sh_ml[w][0][col]);
+  const float Mb = M == kNegInf ? 0.f : M;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) L += sh_ml[w][1][col] * __builtin_amdgcn_exp2f(sh_ml[w][0][col] - Mb);
+  const float f = __builtin_amdgcn_exp2f(mx - Mb);
+#pragma unroll
+  for (int m = 0; m < NB; ++m)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[m][i] *= f;
+#pragma unroll
+  for (int r = 2; r >= 1; r >>= 1) {
+    if (wave >= r && wave < 2 * r) {
+#pragma unroll
+      for (int m = 0; m < NB; ++m)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sh_o[wave - r][m * 16 + i][lane] = o[m][i];
+    }
+    __syncthreads();
+    if (wave < r) {
+#pragma unroll
+      for (int m = 0; m < NB; ++m)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[m][i] += sh_o[wave][m * 16 + i][lane];
+    }
+    __syncthreads();
+  }
+  if (wave != 0 || !live) return;
+
+  if (it.splits > 1) {
+    float* ws = static_cast<float*>(a.ws) + (static_cast<size_t>(slot) * a.hkv + head) * part_floats(kRows, a.d);
+    if (half == 0) {
+      ws[col] = M;
+      ws[kRows + col] = L;
+    }
+    float* wo = ws + 2 * kRows + static_cast<size_t>(col) * a.d;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int d = NB * (8 * (i / 4) + 4 * half + i % 4);
+      if (d < a.d) {
+#pragma unroll
+        for (int m = 0; m < NB; ++m) wo[d + m] = o[m][i];
+      }
+    }
+    return;
+  }
+  const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+  E* op = static_cast<E*>(a.o) + (static_cast<int64_t>(it.t0 + tok) * a.hq + head * a.group + gh) * a.d;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int d = NB * (8 * (i / 4) + 4 * half + i % 4);
+    if (d < a.d) {
+      if constexpr (WIDE) {
+#pragma unroll
+        for (int m = 0; m < NB; ++m) op[d + m] = o[m][i] * inv;
+      } else {
+        uint32_t* ow = reinterpret_cast<uint32_t*>(op + d);
+#pragma unroll
+        for (int m = 0; m < NB; m += 2) ow[m / 2] = pack2<T>(o[m][i] * inv, o[m + 1][i] * inv);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------- join ----
+// Joins the splits of one (sequence, tile, kv head): a wave per row, its lanes
+// over the columns.
+//   M = max_s m_s,  o = sum_s e^(m_s - M) o_s / sum_s e^(m_s - M) l_s
+constexpr int kJoinRows = 8;  // rows of a workgroup
+
+template <typename T, int ROWS, int KEYS>
+__global__ __launch_bounds__(kThreads) void paged_attn_join(PagedAttnArgs a) {
+  using E = typename Elem<T>::type;
+  __shared__ int64_t sh_scan[kWaves];
+  __shared__ int sh_found[5];
+  constexpr int G = ROWS / kJoinRows;
+  const int part = static_cast<int>(blockIdx.x % G);
+  const int head = static_cast<int>(blockIdx.x / G % a.hkv);
+  const int pair = static_cast<int>(blockIdx.x / G / a.hkv);
+  const Item it = find_item<ROWS, KEYS, true>(a, pair, sh_scan, sh_found);
+  if (it.b < 0 || it.splits == 1) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const size_t step = static_cast<size_t>(a.hkv) * part_floats(ROWS, a.d);
+  const float* ws = static_cast<const float*>(a.ws) + (static_cast<size_t>(it.slot) * a.hkv + head) * part_floats(ROWS, a.d);
+  for (int r = part * kJoinRows + wave; r < (part + 1) * kJoinRows; r += kWaves) {
+    const int row = it.tile * ROWS + r;
+    if (row >= it.n * a.group) return;
+    const int tok = row / a.group, gh = row - tok * a.group;
+    float M = kNegInf;
+    for (int s = lane; s < it.splits; s += 64) M = fmaxf(M, ws[s * step + r]);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) M = fmaxf(M, __shfl_xor(M, d));
+    const float Mb = M == kNegInf ? 0.f : M;
+    float L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < it.splits; ++s) {
+      const float* w = ws + s * step;
+      const float f = __builtin_amdgcn_exp2f(w[r] - Mb);
+      L += f * w[ROWS + r];
+      const float* wo = w + 2 * ROWS + static_cast<size_t>(r) * a.d;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (lane + 64 * e < a.d) acc[e] += f * wo[lane + 64 * e];
+    }
+    const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+    E* op = static_cast<E*>(a.o) + (static_cast<int64_t>(it.t0 + tok) * a.hq + head * a.group + gh) * a.d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (lane + 64 * e < a.d) {
+        if constexpr (Elem<T>::wide)
+          op[lane + 64 * e] = acc[e] * inv;
+        else
+          op[lane + 64 * e] = static_cast<E>(pack2<T>(acc[e] * inv, 0.f));
+      }
+  }
+}
+
+template <typename T>
+void launch(const PagedAttnArgs& a, int64_t pairs, hipStream_t s) {
+  const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(a.slots) * a.hkv);
+  if (a.d <= 64)
+    paged_attn_stream<T, 64><<<grid, kThreads, 0, s>>>(a);
+  else if (a.d <= 128)
+    paged_attn_stream<T, 128><<<grid, kThreads, 0, s>>>(a);
+  else
+    paged_attn_stream<T, 256><<<grid, kThreads, 0, s>>>(a);
+  if (a.target > 0)
+    paged_attn_join<T, kRows, kKeys>
+        <<<static_cast<unsigned>(pairs * a.hkv * (kRows / kJoinRows)), kThreads, 0, s>>>(a);
+}
+
+// (sequence, tile) pairs a call can have: every sequence, and the rows behind the last, may end in a partial tile
+int64_t pairs_bound(const PagedAttnArgs& a, int rows) {
+  return static_cast<int64_t>(a.p.T) * (a.hq / a.hkv) / rows + std::min<int64_t>(a.p.B + 1, a.p.T);
+}
+
+void derive(PagedAttnArgs* a) {
+  a->group = a->hq / a->hkv;
+  // enough whole rows to fill the card: no split.  Otherwise about eight
+  // workgroups a compute unit, so that lengths that differ even out.
+  const int64_t full = (static_cast<int64_t>(a->p.T) * a->group + kRows - 1) / kRows * a->hkv;
+  a->target = full >= 4 * kCus ? 0 : static_cast<int>((8 * kCus + a->hkv - 1) / a->hkv);
+  a->min_chunk = 8;
+  a->slots = static_cast<int>(pairs_bound(*a, kRows) + a->target);
+}
+
+}  // namespace
+
+size_t paged_attn_workspace_bytes(const PagedAttnArgs& a0) {
+  PagedAttnArgs a = a0;
+  derive(&a);
+  if (a.target == 0) return 0;
+  return static_cast<size_t>(a.slots) * a.hkv * part_floats(kRows, a.d) * sizeof(float);
+}
+
+void paged_attn(PagedAttnArgs a, hipStream_t s) {
+  derive(&a);
+  const int64_t pairs = pairs_bound(a, kRows);
+  if (a.type == AttnType::kBF16)
+    launch<BF16>(a, pairs, s);
+  else if (a.type == AttnType::kF16)
+    launch<F16>(a, pairs, s);
+  else
+    launch<F32>(a, pairs, s);
+}
+
+}  // namespace kernels
+}  // namespace nnsx
