@@ -21,6 +21,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "kernels/attn.h"
 
@@ -72,18 +73,46 @@ template <>
 __device__ __forceinline__ uint32_t pack2<F16>(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
 }
-// exponent all ones in either half
+// A word's values that are infinite or NaN: their sign bits set in `infinite`
+// (the exponent's bits all ones carry into it), `finite_part` the word with them 0.
 template <typename T>
-__device__ __forceinline__ bool nonfinite2(uint32_t x);
+struct Bits;
 template <>
-__device__ __forceinline__ bool nonfinite2<BF16>(uint32_t x) {
-  return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+struct Bits<BF16> { static constexpr uint32_t exp = 0x7f807f80u, low = 0x00800080u, sign = 0x80008000u; };
+template <>
+struct Bits<F16> { static constexpr uint32_t exp = 0x7c007c00u, low = 0x04000400u, sign = 0x80008000u; };
+template <>
+struct Bits<F32> { static constexpr uint32_t exp = 0x7f800000u, low = 0x00800000u, sign = 0x80000000u; };
+template <typename T>
+__device__ __forceinline__ uint32_t infinite(uint32_t x) {
+  return (x & Bits<T>::exp) + Bits<T>::low;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t finite_part(uint32_t x) {
+  const uint32_t f = infinite<T>(x) & Bits<T>::sign;
+  if constexpr (std::is_same_v<T, F32>) return f ? 0u : x;
+  return x & ~((f >> 15) * 0xffffu);
+}
+// value number e of a word
+template <typename T>
+__device__ __forceinline__ float value_of(uint32_t x, int e);
+template <>
+__device__ __forceinline__ float value_of<BF16>(uint32_t x, int e) {
+  return __uint_as_float(e ? x & 0xffff0000u : x << 16);
 }
 template <>
-__device__ __forceinline__ bool nonfinite2<F16>(uint32_t x) {
-  return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u;
+__device__ __forceinline__ float value_of<F16>(uint32_t x, int e) {
+  return static_cast<float>(__builtin_bit_cast(f16x2, x)[e]);
+}
+template <>
+__device__ __forceinline__ float value_of<F32>(uint32_t x, int) {
+  return __uint_as_float(x);
 }
 
+// the low (0) or high (1) 16 bits of two words, the first's below
+__device__ __forceinline__ uint32_t interleave(uint32_t a, uint32_t b, int high) {
+  return __builtin_amdgcn_perm(b, a, high ? 0x07060302u : 0x05040100u);
+}
 // the other half's value of the same row
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
 
@@ -195,6 +224,10 @@ __device__ Item find_item(const PagedAttnArgs& a, int index, int64_t* sh /* [kWa
   it.split = __builtin_amdgcn_readfirstlane(found[2]);
   it.splits = __builtin_amdgcn_readfirstlane(found[3]);
   it.slot = __builtin_amdgcn_readfirstlane(found[4]);
+  if (PAIRS && (it.slot < 0 || it.slot > a.slots - it.splits)) {  // (offsets that do not ascend: more items than slots)
+    it.b = -1;
+    return it;
+  }
   it.chunk = __builtin_amdgcn_readfirstlane(chunk);
   const Seq s = seq_of<ROWS, KEYS>(a, it.b);
   it.n = __builtin_amdgcn_readfirstlane(s.n);
@@ -231,7 +264,9 @@ struct Elem { using type = uint16_t; static constexpr bool wide = false; };
 template <>
 struct Elem<F32> { using type = float; static constexpr bool wide = true; };
 
-template <typename T, int DP>
+// QUAD: pages hold whole groups of four keys, so four neighbouring rows of V
+// are addressed from the first one's offset.
+template <typename T, int DP, bool QUAD>
 __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) void paged_attn_stream(PagedAttnArgs a) {
   using E = typename Elem<T>::type;
   constexpr bool WIDE = Elem<T>::wide;
@@ -242,6 +277,8 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
   __shared__ int sh_found[5];
   __shared__ float sh_ml[kWaves][2][kRows];
   __shared__ float sh_o[2][NB * 16][64];
+  constexpr bool QLDS = DP * sizeof(E) > 256;
+  __shared__ u32x4 sh_q[QLDS ? KC : 1][64];
 
   const int head = static_cast<int>(blockIdx.x % a.hkv);
   const int slot = static_cast<int>(blockIdx.x / a.hkv);
@@ -276,13 +313,23 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
   const E* vbase = static_cast<const E*>(a.v) + head * a.vh;
   const int* table = a.p.table + static_cast<int64_t>(it.b) * a.p.tstride;
 
-  u32x4 q[KC];
+  // Q: in registers where they suffice, else in LDS (every wave reads the same rows)
+  u32x4 q[QLDS ? 1 : KC];
+  if constexpr (QLDS) {
+    for (int s = wave; s < KC; s += kWaves) {
+      const int d = (2 * s + half) * PIECE;
+      sh_q[s][lane] = live && d < a.d ? *reinterpret_cast<const u32x4*>(qp + d) : (u32x4)(0u);
+    }
+    __syncthreads();
+  } else {
 #pragma unroll
-  for (int s = 0; s < KC; ++s) {
-    const int d = (2 * s + half) * PIECE;
-    q[s] = (u32x4)(0u);
-    if (live && d < a.d) q[s] = *reinterpret_cast<const u32x4*>(qp + d);
+    for (int s = 0; s < KC; ++s) {
+      const int d = (2 * s + half) * PIECE;
+      q[s] = (u32x4)(0u);
+      if (live && d < a.d) q[s] = *reinterpret_cast<const u32x4*>(qp + d);
+    }
   }
+  auto q_piece = [&](int s) { return QLDS ? sh_q[QLDS ? s : 0][lane] : q[QLDS ? 0 : s]; };
 
   f32x16 o[NB];
 #pragma unroll
@@ -296,36 +343,45 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
   uint32_t v[16][VW];
   const int vcol = NB * col;
 
-  // page of this lane's key (lane & 31) in block blk; -1: not there
-  auto page_of = [&](int blk) {
-    const int key = blk * kKeys + col;
-    int id = -1;
-    if (key < it.keys) {
-      id = table[key / a.p.page];
-      if (id < 0 || id >= a.p.pages) id = -1;
-    }
-    return id;
+  // this lane's key (lane & 31) of a block: its rows' offsets, or not there
+  struct KeyRow {
+    int64_t k, v;
+    bool there;
   };
-  auto load_k = [&](int blk, int id) {
-    const int key = blk * kKeys + col;
-    const E* p = kbase + static_cast<int64_t>(id) * a.kp + static_cast<int64_t>(key % a.p.page) * a.kr;
+  auto key_row = [&](int blk) {
+    KeyRow r{0, 0, false};
+    const int key = blk < blk1 ? blk * kKeys + col : it.keys;
+    if (key < it.keys) {
+      const int p = key / a.p.page, off = key - p * a.p.page;
+      const int id = table[p];
+      r.there = id >= 0 && id < a.p.pages;
+      if (r.there) {
+        r.k = id * a.kp + off * a.kr;
+        r.v = id * a.vp + off * a.vr;
+      }
+    }
+    return r;
+  };
+  auto load_k = [&](const KeyRow& r) {
+    const E* p = kbase + r.k;
 #pragma unroll
     for (int s = 0; s < KC; ++s) {
       const int d = (2 * s + half) * PIECE;
       k[s] = (u32x4)(0u);
-      if (id >= 0 && d < a.d) k[s] = *reinterpret_cast<const u32x4*>(p + d);
+      if (r.there && d < a.d) k[s] = *reinterpret_cast<const u32x4*>(p + d);
     }
   };
-  auto load_v = [&](int blk, int id) {
+  auto load_v = [&](const KeyRow& r) {
+    const uint32_t there = static_cast<uint32_t>(__ballot(r.there)) >> (4 * half);
+    int64_t first = 0;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const int kk = 8 * (i / 4) + 4 * half + i % 4;
-      const int kid = __shfl(id, kk);
-      const int key = blk * kKeys + kk;
-      const E* p = vbase + static_cast<int64_t>(kid) * a.vp + static_cast<int64_t>(key % a.p.page) * a.vr + vcol;
+      const int kk = 8 * (i / 4) + i % 4;
+      if (!QUAD || i % 4 == 0) first = __shfl(r.v, kk + 4 * half);
+      const E* p = vbase + first + (QUAD ? (i % 4) * a.vr : 0) + vcol;
 #pragma unroll
       for (int w = 0; w < VW; ++w) v[i][w] = 0u;
-      if (kid >= 0 && vcol < a.d) {
+      if ((there >> kk & 1) && vcol < a.d) {
         if constexpr (VW == 1) {
           v[i][0] = *reinterpret_cast<const uint32_t*>(p);
         } else if constexpr (VW == 2) {
@@ -345,28 +401,27 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
   };
 
   int blk = blk0 + wave;
-  int id = blk < blk1 ? page_of(blk) : -1;
+  KeyRow here = key_row(blk), then = key_row(blk + kWaves);
   if (blk < blk1) {
-    load_k(blk, id);
-    load_v(blk, id);
+    load_k(here);
+    load_v(here);
   }
-  int idn = blk + kWaves < blk1 ? page_of(blk + kWaves) : -1;
   while (blk < blk1) {
     const int next = blk + kWaves;
     const int key0 = blk * kKeys;
-    const uint32_t there = static_cast<uint32_t>(__ballot(id >= 0));  // (lanes 0 .. 31: the block's keys)
+    const uint32_t there = static_cast<uint32_t>(__ballot(here.there));  // (lanes 0 .. 31: the block's keys)
     f32x16 s = (f32x16)(0.f);
     if constexpr (WIDE) {
 #pragma unroll
       for (int i = 0; i < KC; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k[i][e]), __uint_as_float(q[i][e]), s, 0, 0, 0);
+          s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k[i][e]), __uint_as_float(q_piece(i)[e]), s, 0, 0, 0);
     } else {
 #pragma unroll
-      for (int i = 0; i < KC; ++i) s = mfma16<T>(k[i], q[i], s);
+      for (int i = 0; i < KC; ++i) s = mfma16<T>(k[i], q_piece(i), s);
     }
-    if (next < blk1) load_k(next, idn);
+    if (next < blk1) load_k(then);
     // every row of the tile sees every key of the block?
     const bool full = there == 0xffffffffu && __all(!live || (rlo <= key0 && key0 + kKeys <= rhi));
     if (!full) {
@@ -400,46 +455,48 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
     }
 
     // O^T += V^T P^T.  Where a key is hidden from some rows only, its weight
-    // is 0 there, but 0 times an infinite or NaN value is not: such a block is
-    // added key by key, and only to the rows that see the key.
-    bool odd = false;
+    // is 0 there, but 0 times an infinite or NaN value is not: in such a block
+    // those values are taken out of V and added to the rows that see their key.
     if (!full) {
-      bool nf = false;
+      uint32_t inf = 0;
 #pragma unroll
       for (int i = 0; i < 16; ++i)
 #pragma unroll
-        for (int w = 0; w < VW; ++w) {
-          if constexpr (WIDE)
-            nf |= (v[i][w] & 0x7f800000u) == 0x7f800000u;
-          else
-            nf |= nonfinite2<T>(v[i][w]);
-        }
-      odd = __any(nf);
-    }
-    if constexpr (WIDE) {
-      if (!odd) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-#pragma unroll
-          for (int m = 0; m < NB; ++m)
-            o[m] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(v[i][m]), s[i], o[m], 0, 0, 0);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
+        for (int w = 0; w < VW; ++w) inf |= infinite<T>(v[i][w]);
+      if (__any((inf & Bits<T>::sign) != 0)) {
 #pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            const int key = key0 + 8 * (i / 4) + 4 * h + i % 4;
-            const bool sees = key >= rlo && key < rhi && (there >> (key - key0) & 1);
-            const float p = half == h ? s[i] : 0.f;
+        for (int kk = 0; kk < kKeys; ++kk) {
+          if (!(there >> kk & 1)) continue;
+          const int key = key0 + kk;
+          const bool sees = key >= rlo && key < rhi;
+          const E* p = vbase + __shfl(here.v, kk);
 #pragma unroll
-            for (int m = 0; m < NB; ++m) {
-              const float x = half == h ? __uint_as_float(v[i][m]) : 0.f;
-              const f32x16 t = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p, (f32x16)(0.f), 0, 0, 0);
+          for (int i = 0; i < 16; ++i) {
+            const int d = NB * (8 * (i / 4) + 4 * half + i % 4);
+            if (sees && d < a.d) {
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[m][e] = sees ? o[m][e] + t[e] : o[m][e];
+              for (int m = 0; m < NB; m += WIDE ? 1 : 2) {
+                const uint32_t x = *reinterpret_cast<const uint32_t*>(p + d + m);
+                const uint32_t f = infinite<T>(x) & Bits<T>::sign;
+#pragma unroll
+                for (int e = 0; e < (WIDE ? 1 : 2); ++e)
+                  if (f >> (WIDE ? 31 : 15 + 16 * e) & 1) o[m + e][i] += value_of<T>(x, e);
+              }
             }
           }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+          for (int w = 0; w < VW; ++w) v[i][w] = finite_part<T>(v[i][w]);
       }
+    }
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int m = 0; m < NB; ++m)
+          o[m] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(v[i][m]), s[i], o[m], 0, 0, 0);
     } else {
       u32x4 p[2];
 #pragma unroll
@@ -447,45 +504,19 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
 #pragma unroll
         for (int e = 0; e < 4; ++e) p[t][e] = pack2<T>(s[8 * t + 2 * e], s[8 * t + 2 * e + 1]);
 #pragma unroll
-      for (int m = 0; m < NB; ++m) {
-        u32x4 vt[2];
-        constexpr uint32_t kLow = 0x05040100u, kHigh = 0x07060302u;
+      for (int m = 0; m < NB; ++m)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t) {
+          u32x4 vt;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            vt[t][e] = __builtin_amdgcn_perm(v[8 * t + 2 * e + 1][m / 2], v[8 * t + 2 * e][m / 2], m % 2 ? kHigh : kLow);
-        if (!odd) {
-          o[m] = mfma16<T>(vt[0], p[0], o[m]);
-          o[m] = mfma16<T>(vt[1], p[1], o[m]);
-        } else {
-#pragma unroll 1
-          for (int kk = 0; kk < kKeys; ++kk) {
-            const int key = key0 + kk;
-            const bool sees = key >= rlo && key < rhi && (there >> kk & 1);
-            const int i = 4 * (kk / 8) + kk % 4;
-            const uint32_t pick = half == (kk >> 2 & 1) ? (i & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
-            f32x16 t = (f32x16)(0.f);
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              u32x4 va, pa;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t mask = i / 2 == 4 * g + e ? pick : 0u;
-                va[e] = vt[g][e] & mask;
-                pa[e] = p[g][e] & mask;
-              }
-              t = mfma16<T>(va, pa, t);
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[m][e] = sees ? o[m][e] + t[e] : o[m][e];
-          }
+            vt[e] = interleave(v[8 * t + 2 * e][m / 2], v[8 * t + 2 * e + 1][m / 2], m % 2);
+          o[m] = mfma16<T>(vt, p[t], o[m]);
         }
-      }
     }
-    if (next < blk1) load_v(next, idn);
-    id = idn;
-    idn = next + kWaves < blk1 ? page_of(next + kWaves) : -1;
+    if (next < blk1) load_v(then);
+    here = then;
+    then = key_row(next + kWaves);
     blk = next;
   }
   sum += other_half(sum);
@@ -562,69 +593,106 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
 }
 
 // ------------------------------------------------------------------- join ----
-// Joins the splits of one (sequence, tile, kv head): a wave per row, its lanes
-// over the columns.
-//   M = max_s m_s,  o = sum_s e^(m_s - M) o_s / sum_s e^(m_s - M) l_s
-constexpr int kJoinRows = 8;  // rows of a workgroup
+// Joins the splits of one (sequence, tile, kv head):
+//   M = max_s m_s,  o = sum_s e^(m_s - M) o_s / sum_s e^(m_s - M) l_s.
+// LG lanes hold a row's columns, four each; the workgroup's 1024 / LG such
+// groups divide the live rows and, where there are few, a row's splits, whose
+// parts are added through LDS in a fixed order.
+constexpr int kJoinThreads = 1024;
 
-template <typename T, int ROWS, int KEYS>
-__global__ __launch_bounds__(kThreads) void paged_attn_join(PagedAttnArgs a) {
+template <typename T, int ROWS, int KEYS, int LG>
+__global__ __launch_bounds__(kJoinThreads) void paged_attn_join(PagedAttnArgs a) {
   using E = typename Elem<T>::type;
-  __shared__ int64_t sh_scan[kWaves];
+  constexpr int NG = kJoinThreads / LG;
+  __shared__ int64_t sh_scan[kJoinThreads / 64];
   __shared__ int sh_found[5];
-  constexpr int G = ROWS / kJoinRows;
-  const int part = static_cast<int>(blockIdx.x % G);
-  const int head = static_cast<int>(blockIdx.x / G % a.hkv);
-  const int pair = static_cast<int>(blockIdx.x / G / a.hkv);
-  const Item it = find_item<ROWS, KEYS, true>(a, pair, sh_scan, sh_found);
+  __shared__ f32x4 sh_o[NG][LG];
+  __shared__ float sh_l[NG];
+  const int head = static_cast<int>(blockIdx.x % a.hkv);
+  const Item it = find_item<ROWS, KEYS, true>(a, static_cast<int>(blockIdx.x / a.hkv), sh_scan, sh_found);
   if (it.b < 0 || it.splits == 1) return;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lg = threadIdx.x % LG, grp = threadIdx.x / LG;
+  const int live = min(it.n * a.group - it.tile * ROWS, ROWS);
+  int per_row = NG;  // groups of a row: a power of two
+  while (per_row > 1 && per_row * live > NG) per_row >>= 1;
+  const int rows_at_once = NG / per_row, part = grp % per_row;
   const size_t step = static_cast<size_t>(a.hkv) * part_floats(ROWS, a.d);
   const float* ws = static_cast<const float*>(a.ws) + (static_cast<size_t>(it.slot) * a.hkv + head) * part_floats(ROWS, a.d);
-  for (int r = part * kJoinRows + wave; r < (part + 1) * kJoinRows; r += kWaves) {
-    const int row = it.tile * ROWS + r;
-    if (row >= it.n * a.group) return;
-    const int tok = row / a.group, gh = row - tok * a.group;
-    float M = kNegInf;
-    for (int s = lane; s < it.splits; s += 64) M = fmaxf(M, ws[s * step + r]);
+  for (int r0 = 0; r0 < live; r0 += rows_at_once) {
+    const int r = r0 + grp / per_row;
+    f32x4 acc = (f32x4)(0.f);
+    float L = 0.f;
+    if (r < live) {
+      float M = kNegInf;
+      for (int s = lg; s < it.splits; s += LG) M = fmaxf(M, ws[s * step + r]);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) M = fmaxf(M, __shfl_xor(M, d));
-    const float Mb = M == kNegInf ? 0.f : M;
-    float L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < it.splits; ++s) {
-      const float* w = ws + s * step;
-      const float f = __builtin_amdgcn_exp2f(w[r] - Mb);
-      L += f * w[ROWS + r];
-      const float* wo = w + 2 * ROWS + static_cast<size_t>(r) * a.d;
+      for (int d = 1; d < LG; d <<= 1) M = fmaxf(M, __shfl_xor(M, d));
+      if (M == kNegInf) M = 0.f;
+#pragma unroll 8
+      for (int s = part; s < it.splits; s += per_row) {
+        const float* w = ws + s * step;
+        const float f = __builtin_amdgcn_exp2f(w[r] - M);
+        L += f * w[ROWS + r];
+        if (4 * lg < a.d) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(w + 2 * ROWS + static_cast<size_t>(r) * a.d + 4 * lg);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (lane + 64 * e < a.d) acc[e] += f * wo[lane + 64 * e];
-    }
-    const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
-    E* op = static_cast<E*>(a.o) + (static_cast<int64_t>(it.t0 + tok) * a.hq + head * a.group + gh) * a.d;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (lane + 64 * e < a.d) {
-        if constexpr (Elem<T>::wide)
-          op[lane + 64 * e] = acc[e] * inv;
-        else
-          op[lane + 64 * e] = static_cast<E>(pack2<T>(acc[e] * inv, 0.f));
+          for (int e = 0; e < 4; ++e) acc[e] += f * x[e];
+        }
       }
+    }
+    if (per_row > 1) {  // (the same in every thread)
+      __syncthreads();
+      sh_o[grp][lg] = acc;
+      if (lg == 0) sh_l[grp] = L;
+      __syncthreads();
+      if (part == 0)
+        for (int i = 1; i < per_row; ++i) {
+          const f32x4 x = sh_o[grp + i][lg];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] += x[e];
+          L += sh_l[grp + i];
+        }
+    }
+    if (part != 0 || r >= live || 4 * lg >= a.d) continue;
+    const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+    const int row = it.tile * ROWS + r, tok = row / a.group, gh = row - tok * a.group;
+    E* op = static_cast<E*>(a.o) + (static_cast<int64_t>(it.t0 + tok) * a.hq + head * a.group + gh) * a.d + 4 * lg;
+    if constexpr (Elem<T>::wide)
+      *reinterpret_cast<f32x4*>(op) = (f32x4){acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
+    else
+      *reinterpret_cast<u32x2*>(op) = (u32x2){pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv)};
   }
+}
+
+template <typename T, int ROWS, int KEYS>
+void launch_join(const PagedAttnArgs& a, int64_t pairs, hipStream_t s) {
+  const unsigned grid = static_cast<unsigned>(pairs * a.hkv);
+  if (a.d <= 64)
+    paged_attn_join<T, ROWS, KEYS, 16><<<grid, kJoinThreads, 0, s>>>(a);
+  else if (a.d <= 128)
+    paged_attn_join<T, ROWS, KEYS, 32><<<grid, kJoinThreads, 0, s>>>(a);
+  else
+    paged_attn_join<T, ROWS, KEYS, 64><<<grid, kJoinThreads, 0, s>>>(a);
+}
+
+template <typename T, bool QUAD>
+void launch_stream(const PagedAttnArgs& a, hipStream_t s) {
+  const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(a.slots) * a.hkv);
+  if (a.d <= 64)
+    paged_attn_stream<T, 64, QUAD><<<grid, kThreads, 0, s>>>(a);
+  else if (a.d <= 128)
+    paged_attn_stream<T, 128, QUAD><<<grid, kThreads, 0, s>>>(a);
+  else
+    paged_attn_stream<T, 256, QUAD><<<grid, kThreads, 0, s>>>(a);
 }
 
 template <typename T>
 void launch(const PagedAttnArgs& a, int64_t pairs, hipStream_t s) {
-  const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(a.slots) * a.hkv);
-  if (a.d <= 64)
-    paged_attn_stream<T, 64><<<grid, kThreads, 0, s>>>(a);
-  else if (a.d <= 128)
-    paged_attn_stream<T, 128><<<grid, kThreads, 0, s>>>(a);
+  if (a.p.page % 4 == 0)
+    launch_stream<T, true>(a, s);
   else
-    paged_attn_stream<T, 256><<<grid, kThreads, 0, s>>>(a);
-  if (a.target > 0)
-    paged_attn_join<T, kRows, kKeys>
-        <<<static_cast<unsigned>(pairs * a.hkv * (kRows / kJoinRows)), kThreads, 0, s>>>(a);
+    launch_stream<T, false>(a, s);
+  if (a.target > 0) launch_join<T, kRows, kKeys>(a, pairs, s);
 }
 
 // (sequence, tile) pairs a call can have: every sequence, and the rows behind the last, may end in a partial tile
@@ -634,10 +702,10 @@ int64_t pairs_bound(const PagedAttnArgs& a, int rows) {
 
 void derive(PagedAttnArgs* a) {
   a->group = a->hq / a->hkv;
-  // enough whole rows to fill the card: no split.  Otherwise about eight
+  // enough whole rows to fill the card: no split.  Otherwise about four
   // workgroups a compute unit, so that lengths that differ even out.
   const int64_t full = (static_cast<int64_t>(a->p.T) * a->group + kRows - 1) / kRows * a->hkv;
-  a->target = full >= 4 * kCus ? 0 : static_cast<int>((8 * kCus + a->hkv - 1) / a->hkv);
+  a->target = full >= 4 * kCus ? 0 : static_cast<int>((4 * kCus + a->hkv - 1) / a->hkv);
   a->min_chunk = 8;
   a->slots = static_cast<int>(pairs_bound(*a, kRows) + a->target);
 }
