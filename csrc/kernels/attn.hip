@@ -45,6 +45,7 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kRows = 32;   // rows of one item
 constexpr int kKeys = 32;   // keys of one block
 constexpr int kCus = 256;
+constexpr int kFound = 9;   // ints of LDS that find_item passes an item through
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_huge_valf();
 
@@ -145,7 +146,9 @@ __device__ __forceinline__ Seq seq_of(const PagedAttnArgs& a, int b) {
   s.n = max(t1 - s.t0, 0);
   s.len = b < a.p.B ? max(a.p.len[b], 0) : 0;
   s.keys = static_cast<int>(min(static_cast<int64_t>(s.len), static_cast<int64_t>(a.p.width) * a.p.page));
-  s.tiles = static_cast<int>((static_cast<int64_t>(s.n) * a.group + ROWS - 1) / ROWS);
+  const int64_t rows = static_cast<int64_t>(s.n) * a.group;
+  if (rows <= a.rows_lo || rows > a.rows_hi) s.n = 0;  // (another launch's)
+  s.tiles = s.n > 0 ? static_cast<int>((rows + ROWS - 1) / ROWS) : 0;
   const int64_t first = static_cast<int64_t>(s.len) - s.n - a.window + 1;  // first key the first token sees
   const int lo = a.window > 0 ? static_cast<int>(min(max(first, static_cast<int64_t>(0)), static_cast<int64_t>(s.keys))) : 0;
   s.blocks = s.n > 0 ? (s.keys + KEYS - 1) / KEYS - lo / KEYS : 0;
@@ -176,13 +179,14 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t* t
 // PAIRS false: `index` counts items; PAIRS true: (sequence, tile) pairs, and
 // the item's slot is that of the pair's first split
 template <int ROWS, int KEYS, bool PAIRS>
-__device__ Item find_item(const PagedAttnArgs& a, int index, int64_t* sh /* [kWaves] */, int* found /* [5] */) {
+__device__ Item find_item(const PagedAttnArgs& a, int index, int64_t* sh /* [kWaves] */, int* found /* [kFound] */) {
   Item it;
   const int tid = threadIdx.x, nt = blockDim.x, B1 = a.p.B + 1;
   int chunk = 1 << 28;
+  const Seq mine0 = tid < B1 ? seq_of<ROWS, KEYS>(a, tid) : Seq{};
   if (a.target > 0) {
-    int64_t w = 0, total;
-    for (int b = tid; b < B1; b += nt) {
+    int64_t w = static_cast<int64_t>(mine0.tiles) * mine0.blocks, total;
+    for (int b = tid + nt; b < B1; b += nt) {
       const Seq s = seq_of<ROWS, KEYS>(a, b);
       w += static_cast<int64_t>(s.tiles) * s.blocks;
     }
@@ -196,8 +200,9 @@ __device__ Item find_item(const PagedAttnArgs& a, int index, int64_t* sh /* [kWa
     const int b = b0 + tid;
     int64_t mine = 0;
     int tiles = 0, splits = 1;
+    Seq s = mine0;
     if (b < B1) {
-      const Seq s = seq_of<ROWS, KEYS>(a, b);
+      if (b0 > 0) s = seq_of<ROWS, KEYS>(a, b);
       tiles = s.tiles;
       splits = max((s.blocks + chunk - 1) / chunk, 1);
       mine = (static_cast<int64_t>(tiles) << 32) + static_cast<int64_t>(tiles) * splits;
@@ -212,7 +217,11 @@ __device__ Item find_item(const PagedAttnArgs& a, int index, int64_t* sh /* [kWa
       found[1] = tiles - 1 - tile;  // the tiles with the most keys first: the short ones fill the tail
       found[2] = PAIRS ? 0 : rel % splits;
       found[3] = splits;
-      found[4] = first_item + tile * splits + found[2];
+      found[4] = first_item + tile * splits + (PAIRS ? 0 : rel % splits);
+      found[5] = s.n;
+      found[6] = s.t0;
+      found[7] = s.len;
+      found[8] = s.keys;
     }
     carry += total;
     if (index < (PAIRS ? carry >> 32 : carry & 0xffffffff)) break;  // (the same in every thread)
@@ -229,11 +238,10 @@ __device__ Item find_item(const PagedAttnArgs& a, int index, int64_t* sh /* [kWa
     return it;
   }
   it.chunk = __builtin_amdgcn_readfirstlane(chunk);
-  const Seq s = seq_of<ROWS, KEYS>(a, it.b);
-  it.n = __builtin_amdgcn_readfirstlane(s.n);
-  it.t0 = __builtin_amdgcn_readfirstlane(s.t0);
-  it.len = __builtin_amdgcn_readfirstlane(s.len);
-  it.keys = __builtin_amdgcn_readfirstlane(s.keys);
+  it.n = __builtin_amdgcn_readfirstlane(found[5]);
+  it.t0 = __builtin_amdgcn_readfirstlane(found[6]);
+  it.len = __builtin_amdgcn_readfirstlane(found[7]);
+  it.keys = __builtin_amdgcn_readfirstlane(found[8]);
   return it;
 }
 
@@ -274,7 +282,7 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
   constexpr int KC = WIDE ? DP / 8 : DP / 16;  // 16-byte pieces of a key per lane
   constexpr int PIECE = WIDE ? 4 : 8;    // elements of a piece
   __shared__ int64_t sh_scan[kWaves];
-  __shared__ int sh_found[5];
+  __shared__ int sh_found[kFound];
   __shared__ float sh_ml[kWaves][2][kRows];
   __shared__ float sh_o[2][NB * 16][64];
   constexpr bool QLDS = DP * sizeof(E) > 256;
@@ -592,37 +600,317 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
   }
 }
 
+// -------------------------------------------------------------- tile kernel ----
+// Many rows of one sequence: a workgroup of WAVES waves takes 32 rows each and
+// all walk over the same key blocks of 64, staged through LDS in two buffers:
+// the next block's rows are loaded to registers before the current one is
+// worked on and stored after it, with one barrier a block.  K rows are read as
+// 16-byte pieces; V^T comes out of the row-major tile through the transposing
+// LDS read (ds_read_b64_tr_b16: 16 lanes read 4 keys x 16 columns and each gets
+// one column's 4 keys).  Pieces of a row are stored at piece ^ f(row), with f
+// such that the 16 lanes of a read (K: 16 rows, one piece; V: 4 rows, 4 pieces) touch every bank once.
+constexpr int kTileKeys = 64;
+
+template <int DP>
+__device__ __forceinline__ int k_piece(int row, int piece) {  // 16-byte pieces from the tile's start
+  constexpr int P = DP / 8;
+  return row * P + (piece ^ (P >= 16 ? row & 15 : row >> 1 & 7));
+}
+template <int DP>
+__device__ __forceinline__ int v_piece(int row, int piece) {
+  constexpr int P = DP / 8;
+  return row * P + (piece ^ (P >= 16 ? (row & 3) << 2 : (row >> 1 & 1) << 2));
+}
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <typename T, int DP, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile(PagedAttnArgs a) {
+  using E = uint16_t;
+  constexpr int ROWS = WAVES * 32, NB = DP / 32, KC = DP / 16, P = DP / 8;
+  constexpr int PASS = WAVES * 64 / P;                 // rows of a tile that the workgroup loads at once
+  constexpr int PASSES = kTileKeys / PASS;
+  static_assert(PASS * PASSES == kTileKeys && 64 % P == 0 && PASS >= 1, "tile");
+  __shared__ int64_t sh_scan[WAVES];
+  __shared__ int sh_found[kFound];
+  __shared__ u32x4 sh_k[2][kTileKeys * P];
+  __shared__ u32x4 sh_v[2][kTileKeys * P];
+
+  const int head = static_cast<int>(blockIdx.x % a.hkv);
+  const int slot = static_cast<int>(blockIdx.x / a.hkv);
+  const Item it = find_item<ROWS, kTileKeys, false>(a, slot, sh_scan, sh_found);
+  if (it.b < 0) return;
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int rows = it.n * a.group;
+  const int row = it.tile * ROWS + wave * 32 + col;
+  const bool live = row < rows;
+  const int tok = row / a.group, gh = row - tok * a.group;
+  int rlo, rhi, tlo, thi, wlo, whi;  // keys of this lane's row, of the tile, of the wave
+  key_range(a, it, tok, tok, &rlo, &rhi);
+  if (!live) rhi = rlo = 0;
+  {
+    const int f = it.tile * ROWS, l = min(f + ROWS, rows) - 1;
+    key_range(a, it, f / a.group, l / a.group, &tlo, &thi);
+    const int wf = f + wave * 32, wl = min(wf + 32, rows) - 1;
+    wlo = whi = 0;
+    if (wf < rows) key_range(a, it, wf / a.group, wl / a.group, &wlo, &whi);
+  }
+  int blk0 = tlo / kTileKeys, blk1 = (thi + kTileKeys - 1) / kTileKeys;
+  {
+    const int64_t s0 = blk0 + static_cast<int64_t>(it.split) * it.chunk;
+    const int64_t s1 = s0 + it.chunk;
+    blk0 = static_cast<int>(min(s0, static_cast<int64_t>(blk1)));
+    blk1 = static_cast<int>(min(s1, static_cast<int64_t>(blk1)));
+  }
+
+  const E* qp = static_cast<const E*>(a.q) + static_cast<int64_t>(it.t0 + tok) * a.qt +
+                static_cast<int64_t>(head * a.group + gh) * a.qh;
+  const E* kbase = static_cast<const E*>(a.k) + head * a.kh;
+  const E* vbase = static_cast<const E*>(a.v) + head * a.vh;
+  const int* table = a.p.table + static_cast<int64_t>(it.b) * a.p.tstride;
+
+  u32x4 q[KC];
+#pragma unroll
+  for (int s = 0; s < KC; ++s) {
+    const int d = (2 * s + half) * 8;
+    q[s] = (u32x4)(0u);
+    if (live && d < a.d) q[s] = *reinterpret_cast<const u32x4*>(qp + d);
+  }
+  f32x16 o[NB];
+#pragma unroll
+  for (int m = 0; m < NB; ++m) o[m] = (f32x16)(0.f);
+  float mx = kNegInf, sum = 0.f;
+  const float c = a.scale * kLog2e;
+
+  // lane i: key i of a block
+  struct KeyRow {
+    int64_t k, v;
+    bool there;
+  };
+  auto key_row = [&](int blk) {
+    KeyRow r{0, 0, false};
+    const int key = blk < blk1 ? blk * kTileKeys + lane : it.keys;
+    if (key < it.keys) {
+      const int p = key / a.p.page, off = key - p * a.p.page;
+      const int id = table[p];
+      r.there = id >= 0 && id < a.p.pages;
+      if (r.there) {
+        r.k = id * a.kp + off * a.kr;
+        r.v = id * a.vp + off * a.vr;
+      }
+    }
+    return r;
+  };
+  u32x4 kr[PASSES], vr[PASSES];
+  const int lrow = threadIdx.x / P, piece = threadIdx.x % P;
+  auto load = [&](const KeyRow& r) {
+    const uint64_t there = __ballot(r.there);
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int x = i * PASS + lrow;
+      const E* kp = kbase + __shfl(r.k, x) + piece * 8;
+      const E* vp = vbase + __shfl(r.v, x) + piece * 8;
+      kr[i] = vr[i] = (u32x4)(0u);
+      if ((there >> x & 1) && piece * 8 < a.d) {
+        kr[i] = *reinterpret_cast<const u32x4*>(kp);
+        vr[i] = *reinterpret_cast<const u32x4*>(vp);
+      }
+    }
+  };
+  auto store = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int x = i * PASS + lrow;
+      sh_k[buf][k_piece<DP>(x, piece)] = kr[i];
+      sh_v[buf][v_piece<DP>(x, piece)] = vr[i];
+    }
+  };
+
+  auto block = [&](auto masked, int buf, int key0, uint64_t there) {
+    constexpr bool MASKED = decltype(masked)::value;
+    f32x16 s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      s[b] = (f32x16)(0.f);
+#pragma unroll
+      for (int i = 0; i < KC; ++i) s[b] = mfma16<T>(sh_k[buf][k_piece<DP>(32 * b + col, 2 * i + half)], q[i], s[b]);
+    }
+    if constexpr (MASKED) {
+      const int lo = rlo - key0 - 4 * half, hi = rhi - key0 - 4 * half;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const uint32_t bits = static_cast<uint32_t>(there >> (32 * b)) >> (4 * half);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int kk = 8 * (i / 4) + i % 4;
+          if (!(32 * b + kk >= lo && 32 * b + kk < hi && (bits >> kk & 1))) s[b][i] = kNegInf;
+        }
+      }
+    }
+    float bm = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int i = 1; i < 16; ++i) bm = fmaxf(bm, fmaxf(s[0][i], s[1][i]));
+    bm = fmaxf(bm, other_half(bm));
+    const float nm = fmaxf(mx, bm * c);
+    const float base = MASKED && nm == kNegInf ? 0.f : nm;
+    if (__any(nm > mx)) {
+      const float f = __builtin_amdgcn_exp2f(mx - base);
+      sum *= f;
+#pragma unroll
+      for (int m = 0; m < NB; ++m)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[m][i] *= f;
+      mx = nm;
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[b][i] = __builtin_amdgcn_exp2f(s[b][i] * c - base);
+        sum += s[b][i];
+      }
+    uint32_t inf = 0;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      u32x4 p;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[e] = pack2<T>(s[t / 2][8 * (t % 2) + 2 * e], s[t / 2][8 * (t % 2) + 2 * e + 1]);
+#pragma unroll
+      for (int m = 0; m < NB; ++m) {
+        u32x4 vt;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const int key = 16 * t + 8 * g + 4 * half + (lane & 15) / 4;
+          const int at = v_piece<DP>(key, 4 * m + 2 * (lane >> 4 & 1) + (lane & 3) / 2) * 8 + (lane & 1) * 4;
+          const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s16x4*)(reinterpret_cast<E*>(sh_v[buf]) + at));
+          const u32x2 w = __builtin_bit_cast(u32x2, x);
+          vt[2 * g] = w[0];
+          vt[2 * g + 1] = w[1];
+        }
+        if constexpr (MASKED) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            inf |= infinite<T>(vt[e]);
+            vt[e] = finite_part<T>(vt[e]);
+          }
+        }
+        o[m] = mfma16<T>(vt, p, o[m]);
+      }
+    }
+    if constexpr (MASKED) {  // infinite and NaN values: to the rows that see their key (as in the stream kernel)
+      if (__any((inf & Bits<T>::sign) != 0)) {
+#pragma unroll 1
+        for (int kk = 0; kk < kTileKeys; ++kk) {
+          const bool sees = key0 + kk >= rlo && key0 + kk < rhi && (there >> kk & 1);
+#pragma unroll
+          for (int m = 0; m < NB; ++m)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const int d = 32 * m + 8 * (i / 4) + 4 * half + i % 4;
+              const uint32_t x = reinterpret_cast<const uint32_t*>(sh_v[buf])[v_piece<DP>(kk, d / 8) * 4 + d % 8 / 2];
+              const uint32_t f = sees ? infinite<T>(x) & Bits<T>::sign : 0u;
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (f >> (15 + 16 * e) & 1) o[m][i + e] += value_of<T>(x, e);
+            }
+        }
+      }
+    }
+  };
+
+  KeyRow next = key_row(blk0);
+  uint64_t there_next = __ballot(next.there);
+  if (blk0 < blk1) {
+    load(next);
+    store(0);
+  }
+  next = key_row(blk0 + 1);
+  for (int blk = blk0; blk < blk1; ++blk) {
+    const int buf = (blk - blk0) & 1, key0 = blk * kTileKeys;
+    const uint64_t there = there_next;
+    __syncthreads();  // this block is stored, the other buffer read
+    const bool more = blk + 1 < blk1;
+    if (more) load(next);
+    there_next = __ballot(next.there);
+    next = key_row(blk + 2);
+    if (key0 < whi && key0 + kTileKeys > wlo) {
+      if (there == ~0ull && __all(!live || (rlo <= key0 && key0 + kTileKeys <= rhi)))
+        block(std::false_type{}, buf, key0, there);
+      else
+        block(std::true_type{}, buf, key0, there);
+    }
+    if (more) store(buf ^ 1);
+  }
+  sum += other_half(sum);
+  if (!live) return;
+
+  if (it.splits > 1) {
+    float* ws = static_cast<float*>(a.ws) + (static_cast<size_t>(slot) * a.hkv + head) * part_floats(ROWS, a.d);
+    const int r = wave * 32 + col;
+    if (half == 0) {
+      ws[r] = mx;
+      ws[ROWS + r] = sum;
+    }
+    float* wo = ws + 2 * ROWS + static_cast<size_t>(r) * a.d;
+#pragma unroll
+    for (int m = 0; m < NB; ++m)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const int d = 32 * m + 2 * i + 4 * half;
+        if (d < a.d) *reinterpret_cast<f32x4*>(wo + d) = (f32x4){o[m][i], o[m][i + 1], o[m][i + 2], o[m][i + 3]};
+      }
+    return;
+  }
+  const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+  E* op = static_cast<E*>(a.o) + (static_cast<int64_t>(it.t0 + tok) * a.hq + head * a.group + gh) * a.d;
+#pragma unroll
+  for (int m = 0; m < NB; ++m)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int d = 32 * m + 2 * i + 4 * half;
+      if (d < a.d)
+        *reinterpret_cast<u32x2*>(op + d) = (u32x2){pack2<T>(o[m][i] * inv, o[m][i + 1] * inv),
+                                                    pack2<T>(o[m][i + 2] * inv, o[m][i + 3] * inv)};
+    }
+}
+
 // ------------------------------------------------------------------- join ----
 // Joins the splits of one (sequence, tile, kv head):
 //   M = max_s m_s,  o = sum_s e^(m_s - M) o_s / sum_s e^(m_s - M) l_s.
-// LG lanes hold a row's columns, four each; the workgroup's 1024 / LG such
+// LG lanes hold a row's columns, four each; the workgroup's 256 / LG such
 // groups divide the live rows and, where there are few, a row's splits, whose
-// parts are added through LDS in a fixed order.
-constexpr int kJoinThreads = 1024;
+// parts are added through LDS in a fixed order.  blockIdx.y takes every
+// gridDim.y-th row: few pairs are spread over more workgroups.
+constexpr int kJoinThreads = 256;
 
 template <typename T, int ROWS, int KEYS, int LG>
 __global__ __launch_bounds__(kJoinThreads) void paged_attn_join(PagedAttnArgs a) {
   using E = typename Elem<T>::type;
   constexpr int NG = kJoinThreads / LG;
   __shared__ int64_t sh_scan[kJoinThreads / 64];
-  __shared__ int sh_found[5];
+  __shared__ int sh_found[kFound];
   __shared__ f32x4 sh_o[NG][LG];
   __shared__ float sh_l[NG];
   const int head = static_cast<int>(blockIdx.x % a.hkv);
   const Item it = find_item<ROWS, KEYS, true>(a, static_cast<int>(blockIdx.x / a.hkv), sh_scan, sh_found);
   if (it.b < 0 || it.splits == 1) return;
   const int lg = threadIdx.x % LG, grp = threadIdx.x / LG;
-  const int live = min(it.n * a.group - it.tile * ROWS, ROWS);
+  const int all = min(it.n * a.group - it.tile * ROWS, ROWS), apart = static_cast<int>(gridDim.y);
+  const int live = (all - static_cast<int>(blockIdx.y) + apart - 1) / apart;  // rows of this workgroup
+  if (live <= 0) return;
   int per_row = NG;  // groups of a row: a power of two
   while (per_row > 1 && per_row * live > NG) per_row >>= 1;
   const int rows_at_once = NG / per_row, part = grp % per_row;
   const size_t step = static_cast<size_t>(a.hkv) * part_floats(ROWS, a.d);
   const float* ws = static_cast<const float*>(a.ws) + (static_cast<size_t>(it.slot) * a.hkv + head) * part_floats(ROWS, a.d);
   for (int r0 = 0; r0 < live; r0 += rows_at_once) {
-    const int r = r0 + grp / per_row;
+    const int i0 = r0 + grp / per_row, r = i0 * apart + static_cast<int>(blockIdx.y);
     f32x4 acc = (f32x4)(0.f);
     float L = 0.f;
-    if (r < live) {
+    if (i0 < live) {
       float M = kNegInf;
       for (int s = lg; s < it.splits; s += LG) M = fmaxf(M, ws[s * step + r]);
 #pragma unroll
@@ -653,7 +941,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_attn_join(PagedAttnArgs a)
           L += sh_l[grp + i];
         }
     }
-    if (part != 0 || r >= live || 4 * lg >= a.d) continue;
+    if (part != 0 || i0 >= live || 4 * lg >= a.d) continue;
     const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
     const int row = it.tile * ROWS + r, tok = row / a.group, gh = row - tok * a.group;
     E* op = static_cast<E*>(a.o) + (static_cast<int64_t>(it.t0 + tok) * a.hq + head * a.group + gh) * a.d + 4 * lg;
@@ -666,7 +954,8 @@ __global__ __launch_bounds__(kJoinThreads) void paged_attn_join(PagedAttnArgs a)
 
 template <typename T, int ROWS, int KEYS>
 void launch_join(const PagedAttnArgs& a, int64_t pairs, hipStream_t s) {
-  const unsigned grid = static_cast<unsigned>(pairs * a.hkv);
+  const int64_t wgs = pairs * a.hkv;
+  const dim3 grid(static_cast<unsigned>(wgs), static_cast<unsigned>(std::clamp<int64_t>(4 * kCus / wgs, 1, ROWS)));
   if (a.d <= 64)
     paged_attn_join<T, ROWS, KEYS, 16><<<grid, kJoinThreads, 0, s>>>(a);
   else if (a.d <= 128)
@@ -686,48 +975,101 @@ void launch_stream(const PagedAttnArgs& a, hipStream_t s) {
     paged_attn_stream<T, 256, QUAD><<<grid, kThreads, 0, s>>>(a);
 }
 
-template <typename T>
-void launch(const PagedAttnArgs& a, int64_t pairs, hipStream_t s) {
-  if (a.p.page % 4 == 0)
-    launch_stream<T, true>(a, s);
-  else
-    launch_stream<T, false>(a, s);
-  if (a.target > 0) launch_join<T, kRows, kKeys>(a, pairs, s);
-}
-
 // (sequence, tile) pairs a call can have: every sequence, and the rows behind the last, may end in a partial tile
 int64_t pairs_bound(const PagedAttnArgs& a, int rows) {
-  return static_cast<int64_t>(a.p.T) * (a.hq / a.hkv) / rows + std::min<int64_t>(a.p.B + 1, a.p.T);
+  return static_cast<int64_t>(a.p.T) * a.group / rows + std::min<int64_t>(a.p.B + 1, a.p.T);
 }
 
-void derive(PagedAttnArgs* a) {
-  a->group = a->hq / a->hkv;
-  // enough whole rows to fill the card: no split.  Otherwise about four
-  // workgroups a compute unit, so that lengths that differ even out.
-  const int64_t full = (static_cast<int64_t>(a->p.T) * a->group + kRows - 1) / kRows * a->hkv;
-  a->target = full >= 4 * kCus ? 0 : static_cast<int>((4 * kCus + a->hkv - 1) / a->hkv);
-  a->min_chunk = 8;
-  a->slots = static_cast<int>(pairs_bound(*a, kRows) + a->target);
+int tile_rows(const PagedAttnArgs& a) { return a.d <= 128 ? 256 : 128; }
+
+// One launch of either kernel: which sequences it takes (by their rows), how
+// its keys are split, its scratch memory.  Enough whole tiles to fill the card:
+// no split.  Otherwise about `per_cu` workgroups a compute unit, of at least `min_chunk` key blocks.
+PagedAttnArgs part_of(const PagedAttnArgs& a0, int rows, int rows_lo, int rows_hi, int per_cu, int min_chunk) {
+  PagedAttnArgs a = a0;
+  a.rows_lo = rows_lo;
+  a.rows_hi = rows_hi;
+  const int64_t full = (static_cast<int64_t>(a.p.T) * a.group + rows - 1) / rows * a.hkv;
+  a.target = full >= 2 * per_cu * kCus ? 0 : (per_cu * kCus + a.hkv - 1) / a.hkv;
+  a.min_chunk = min_chunk;
+  a.slots = static_cast<int>(pairs_bound(a, rows) + a.target);
+  return a;
+}
+
+size_t part_bytes(const PagedAttnArgs& a, int rows) {
+  return a.target == 0 ? 0 : static_cast<size_t>(a.slots) * a.hkv * part_floats(rows, a.d) * sizeof(float);
+}
+
+constexpr int kAllRows = 0x7fffffff;
+// Rows of a sequence up to which the stream kernel takes it
+constexpr int kStreamRows = 64;
+
+struct Plan {
+  bool stream, tile;
+  PagedAttnArgs s, t;
+};
+
+Plan plan_of(PagedAttnArgs a) {
+  a.group = a.hq / a.hkv;
+  Plan p;
+  // One token a sequence on average: the stream kernel takes every sequence.
+  // A single sequence is one kernel's.  Else both run, each on its own sequences.
+  if (a.type == AttnType::kF32 || a.p.T <= a.p.B)
+    p.tile = false;
+  else
+    p.tile = a.p.B > 1 || static_cast<int64_t>(a.p.T) * a.group > kStreamRows;
+  p.stream = !p.tile || a.p.B > 1;
+  p.s = part_of(a, kRows, 0, p.tile ? kStreamRows : kAllRows, 4, 4);
+  p.t = part_of(a, tile_rows(a), p.stream ? kStreamRows : 0, kAllRows, 1, 4);
+  p.t.ws = static_cast<char*>(a.ws) + (p.stream ? part_bytes(p.s, kRows) : 0);
+  return p;
+}
+
+template <typename T>
+void launch(const Plan& p, hipStream_t s) {
+  if constexpr (!Elem<T>::wide) {
+    if (p.tile) {
+      const PagedAttnArgs& a = p.t;
+      const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(a.slots) * a.hkv);
+      if (a.d <= 64)
+        paged_attn_tile<T, 64, 8><<<grid, 512, 0, s>>>(a);
+      else if (a.d <= 128)
+        paged_attn_tile<T, 128, 8><<<grid, 512, 0, s>>>(a);
+      else
+        paged_attn_tile<T, 256, 4><<<grid, 256, 0, s>>>(a);
+      if (a.target > 0) {
+        if (a.d <= 128)
+          launch_join<T, 256, kTileKeys>(a, pairs_bound(a, 256), s);
+        else
+          launch_join<T, 128, kTileKeys>(a, pairs_bound(a, 128), s);
+      }
+    }
+  }
+  if (p.stream) {
+    const PagedAttnArgs& a = p.s;
+    if (a.p.page % 4 == 0)
+      launch_stream<T, true>(a, s);
+    else
+      launch_stream<T, false>(a, s);
+    if (a.target > 0) launch_join<T, kRows, kKeys>(a, pairs_bound(a, kRows), s);
+  }
 }
 
 }  // namespace
 
-size_t paged_attn_workspace_bytes(const PagedAttnArgs& a0) {
-  PagedAttnArgs a = a0;
-  derive(&a);
-  if (a.target == 0) return 0;
-  return static_cast<size_t>(a.slots) * a.hkv * part_floats(kRows, a.d) * sizeof(float);
+size_t paged_attn_workspace_bytes(const PagedAttnArgs& a) {
+  const Plan p = plan_of(a);
+  return (p.stream ? part_bytes(p.s, kRows) : 0) + (p.tile ? part_bytes(p.t, tile_rows(a)) : 0);
 }
 
-void paged_attn(PagedAttnArgs a, hipStream_t s) {
-  derive(&a);
-  const int64_t pairs = pairs_bound(a, kRows);
+void paged_attn(const PagedAttnArgs& a, hipStream_t s) {
+  const Plan p = plan_of(a);
   if (a.type == AttnType::kBF16)
-    launch<BF16>(a, pairs, s);
+    launch<BF16>(p, s);
   else if (a.type == AttnType::kF16)
-    launch<F16>(a, pairs, s);
+    launch<F16>(p, s);
   else
-    launch<F32>(a, pairs, s);
+    launch<F32>(p, s);
 }
 
 }  // namespace kernels
