@@ -114,8 +114,17 @@ __device__ __forceinline__ float value_of<F32>(uint32_t x, int) {
 __device__ __forceinline__ uint32_t interleave(uint32_t a, uint32_t b, int high) {
   return __builtin_amdgcn_perm(b, a, high ? 0x07060302u : 0x05040100u);
 }
-// the other half's value of the same row
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+// max(a, b) as one instruction (fmaxf first quiets both operands); a NaN loses
+__device__ __forceinline__ float max2(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, __builtin_huge_valf()); }
+// over the two lanes of a row, 32 apart
+__device__ __forceinline__ float row_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return max2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float row_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 
 // ------------------------------------------------------------------- plan ----
 // Work is cut into items: (sequence, tile of rows, split of its key blocks).
@@ -443,8 +452,8 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
     }
     float bm = s[0];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) bm = fmaxf(bm, s[i]);
-    bm = fmaxf(bm, other_half(bm));
+    for (int i = 1; i < 16; ++i) bm = max2(bm, s[i]);
+    bm = row_max(bm);
     const float nm = fmaxf(mx, bm * c);
     const float base = nm == kNegInf ? 0.f : nm;  // (a row that has seen nothing yet)
     if (__any(nm > mx)) {
@@ -527,7 +536,7 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
     then = key_row(next + kWaves);
     blk = next;
   }
-  sum += other_half(sum);
+  sum = row_sum(sum);
 
   // join the waves: a common maximum, then O in two rounds (2, 3 -> 0, 1; 1 -> 0)
   if (half == 0) {
@@ -611,18 +620,19 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
 // such that the 16 lanes of a read (K: 16 rows, one piece; V: 4 rows, 4 pieces) touch every bank once.
 constexpr int kTileKeys = 64;
 
+// What piece numbers of a row are combined with (exclusive or).  A row of 128
+// bytes shares the 256 bytes that the banks hold with its neighbour.
 template <int DP>
-__device__ __forceinline__ int k_piece(int row, int piece) {  // 16-byte pieces from the tile's start
-  constexpr int P = DP / 8;
-  return row * P + (piece ^ (P >= 16 ? row & 15 : row >> 1 & 7));
+__device__ __forceinline__ int k_turn(int row) {
+  return DP >= 128 ? row & 15 : row >> 1 & 7;
 }
 template <int DP>
-__device__ __forceinline__ int v_piece(int row, int piece) {
-  constexpr int P = DP / 8;
-  return row * P + (piece ^ (P >= 16 ? (row & 3) << 2 : (row >> 1 & 1) << 2));
+__device__ __forceinline__ int v_turn(int row) {
+  return DP >= 128 ? (row & 3) << 2 : (row >> 1 & 1) << 2;
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+#define NNSX_LDS __attribute__((address_space(3)))
 
 template <typename T, int DP, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile(PagedAttnArgs a) {
@@ -633,8 +643,10 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
   static_assert(PASS * PASSES == kTileKeys && 64 % P == 0 && PASS >= 1, "tile");
   __shared__ int64_t sh_scan[WAVES];
   __shared__ int sh_found[kFound];
-  __shared__ u32x4 sh_k[2][kTileKeys * P];
-  __shared__ u32x4 sh_v[2][kTileKeys * P];
+  // K and V of two blocks; rows are aligned to their size, so that pieces of a row are reached by exclusive or
+  constexpr int ROW = DP * 2, TILE = kTileKeys * ROW;
+  __shared__ __attribute__((aligned(1024))) char sh_kv[4 * TILE];
+  const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((NNSX_LDS char*)sh_kv));
 
   const int head = static_cast<int>(blockIdx.x % a.hkv);
   const int slot = static_cast<int>(blockIdx.x / a.hkv);
@@ -705,6 +717,11 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
   };
   u32x4 kr[PASSES], vr[PASSES];
   const int lrow = threadIdx.x / P, piece = threadIdx.x % P;
+  // addresses in a block (K at 0, V at TILE): this lane's pieces to store, and to read
+  // (passes are a multiple of 16 rows or, for 256 columns, 8: each has its own turn)
+  const uint32_t kread = col * ROW + ((half ^ k_turn<DP>(col)) << 4);
+  const int vrow = 4 * half + (lane & 15) / 4;
+  const uint32_t vread = TILE + vrow * ROW + (((2 * (lane >> 4 & 1) + (lane & 3) / 2) ^ v_turn<DP>(vrow)) << 4) + (lane & 1) * 8;
   auto load = [&](const KeyRow& r) {
     const uint64_t there = __ballot(r.there);
 #pragma unroll
@@ -723,20 +740,21 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
       const int x = i * PASS + lrow;
-      sh_k[buf][k_piece<DP>(x, piece)] = kr[i];
-      sh_v[buf][v_piece<DP>(x, piece)] = vr[i];
+      const uint32_t at = lds + buf * 2 * TILE + x * ROW;
+      *(NNSX_LDS u32x4*)(at + ((piece ^ k_turn<DP>(x)) << 4)) = kr[i];
+      *(NNSX_LDS u32x4*)(at + TILE + ((piece ^ v_turn<DP>(x)) << 4)) = vr[i];
     }
   };
 
   auto block = [&](auto masked, int buf, int key0, uint64_t there) {
     constexpr bool MASKED = decltype(masked)::value;
+    const uint32_t kat = lds + buf * 2 * TILE + kread, vat = lds + buf * 2 * TILE + vread;
     f32x16 s[2];
+    s[0] = s[1] = (f32x16)(0.f);
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      s[b] = (f32x16)(0.f);
+    for (int i = 0; i < KC; ++i)
 #pragma unroll
-      for (int i = 0; i < KC; ++i) s[b] = mfma16<T>(sh_k[buf][k_piece<DP>(32 * b + col, 2 * i + half)], q[i], s[b]);
-    }
+      for (int b = 0; b < 2; ++b) s[b] = mfma16<T>(*(NNSX_LDS u32x4*)((kat ^ i << 5) + b * 32 * ROW), q[i], s[b]);
     if constexpr (MASKED) {
       const int lo = rlo - key0 - 4 * half, hi = rhi - key0 - 4 * half;
 #pragma unroll
@@ -749,14 +767,19 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
         }
       }
     }
-    float bm = fmaxf(s[0][0], s[1][0]);
+    float bm0 = s[0][0], bm1 = s[1][0];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) bm = fmaxf(bm, fmaxf(s[0][i], s[1][i]));
-    bm = fmaxf(bm, other_half(bm));
+    for (int i = 1; i < 16; ++i) {
+      bm0 = max2(bm0, s[0][i]);
+      bm1 = max2(bm1, s[1][i]);
+    }
+    const float bm = row_max(max2(bm0, bm1));
     const float nm = fmaxf(mx, bm * c);
-    const float base = MASKED && nm == kNegInf ? 0.f : nm;
-    if (__any(nm > mx)) {
-      const float f = __builtin_amdgcn_exp2f(mx - base);
+    // the maximum that weights are relative to follows only steps of more than
+    // 2^8: weights stay within [0, 256], far from any type's range, and the
+    // rescale of O is rare (without this 10 % slower)
+    if (__any(nm > mx + 8.f)) {
+      const float f = __builtin_amdgcn_exp2f(mx - (nm == kNegInf ? 0.f : nm));
       sum *= f;
 #pragma unroll
       for (int m = 0; m < NB; ++m)
@@ -764,6 +787,7 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
         for (int i = 0; i < 16; ++i) o[m][i] *= f;
       mx = nm;
     }
+    const float base = mx == kNegInf ? 0.f : mx;  // (a row that has seen nothing yet)
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -782,10 +806,8 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
         u32x4 vt;
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          const int key = 16 * t + 8 * g + 4 * half + (lane & 15) / 4;
-          const int at = v_piece<DP>(key, 4 * m + 2 * (lane >> 4 & 1) + (lane & 3) / 2) * 8 + (lane & 1) * 4;
-          const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) s16x4*)(reinterpret_cast<E*>(sh_v[buf]) + at));
+          const s16x4 x =
+              __builtin_amdgcn_ds_read_tr16_b64_v4i16((NNSX_LDS s16x4*)((vat ^ m << 6) + (16 * t + 8 * g) * ROW));
           const u32x2 w = __builtin_bit_cast(u32x2, x);
           vt[2 * g] = w[0];
           vt[2 * g + 1] = w[1];
@@ -810,7 +832,8 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
               const int d = 32 * m + 8 * (i / 4) + 4 * half + i % 4;
-              const uint32_t x = reinterpret_cast<const uint32_t*>(sh_v[buf])[v_piece<DP>(kk, d / 8) * 4 + d % 8 / 2];
+              const uint32_t x = *(NNSX_LDS uint32_t*)(lds + buf * 2 * TILE + TILE + kk * ROW +
+                                                       ((d / 8 ^ v_turn<DP>(kk)) << 4) + d % 8 * 2);
               const uint32_t f = sees ? infinite<T>(x) & Bits<T>::sign : 0u;
 #pragma unroll
               for (int e = 0; e < 2; ++e)
@@ -844,7 +867,7 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
     }
     if (more) store(buf ^ 1);
   }
-  sum += other_half(sum);
+  sum = row_sum(sum);
   if (!live) return;
 
   if (it.splits > 1) {
