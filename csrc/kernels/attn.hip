@@ -646,6 +646,7 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
   // K and V of two blocks; rows are aligned to their size, so that pieces of a row are reached by exclusive or
   constexpr int ROW = DP * 2, TILE = kTileKeys * ROW;
   __shared__ __attribute__((aligned(1024))) char sh_kv[4 * TILE];
+  __shared__ int sh_inf[2];
   const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((NNSX_LDS char*)sh_kv));
 
   const int head = static_cast<int>(blockIdx.x % a.hkv);
@@ -659,15 +660,22 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
   const int row = it.tile * ROWS + wave * 32 + col;
   const bool live = row < rows;
   const int tok = row / a.group, gh = row - tok * a.group;
-  int rlo, rhi, tlo, thi, wlo, whi;  // keys of this lane's row, of the tile, of the wave
+  // keys that this lane's row sees; that some (lo, hi) and that every row (in_lo,
+  // in_hi) of the tile (t) and of the wave (w) sees
+  int rlo, rhi, tlo, thi, t_in_lo, t_in_hi, wlo = 0, whi = 0, w_in_lo = 0, w_in_hi = 0, x;
   key_range(a, it, tok, tok, &rlo, &rhi);
   if (!live) rhi = rlo = 0;
   {
     const int f = it.tile * ROWS, l = min(f + ROWS, rows) - 1;
     key_range(a, it, f / a.group, l / a.group, &tlo, &thi);
+    key_range(a, it, f / a.group, f / a.group, &x, &t_in_hi);
+    key_range(a, it, l / a.group, l / a.group, &t_in_lo, &x);
     const int wf = f + wave * 32, wl = min(wf + 32, rows) - 1;
-    wlo = whi = 0;
-    if (wf < rows) key_range(a, it, wf / a.group, wl / a.group, &wlo, &whi);
+    if (wf < rows) {
+      key_range(a, it, wf / a.group, wl / a.group, &wlo, &whi);
+      key_range(a, it, wf / a.group, wf / a.group, &x, &w_in_hi);
+      key_range(a, it, wl / a.group, wl / a.group, &w_in_lo, &x);
+    }
   }
   int blk0 = tlo / kTileKeys, blk1 = (thi + kTileKeys - 1) / kTileKeys;
   {
@@ -736,7 +744,16 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
       }
     }
   };
-  auto store = [&](int buf) {
+  // check: a key of the block is hidden from some row of the tile; then infinite and NaN values are flagged
+  auto store = [&](int buf, bool check) {
+    if (check) {
+      uint32_t inf = 0;
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) inf |= infinite<T>(vr[i][e]);
+      if (inf & Bits<T>::sign) sh_inf[buf] = 1;
+    }
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
       const int x = i * PASS + lrow;
@@ -746,109 +763,44 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
     }
   };
 
-  auto block = [&](auto masked, int buf, int key0, uint64_t there) {
-    constexpr bool MASKED = decltype(masked)::value;
-    const uint32_t kat = lds + buf * 2 * TILE + kread, vat = lds + buf * 2 * TILE + vread;
-    f32x16 s[2];
-    s[0] = s[1] = (f32x16)(0.f);
-#pragma unroll
-    for (int i = 0; i < KC; ++i)
-#pragma unroll
-      for (int b = 0; b < 2; ++b) s[b] = mfma16<T>(*(NNSX_LDS u32x4*)((kat ^ i << 5) + b * 32 * ROW), q[i], s[b]);
-    if constexpr (MASKED) {
-      const int lo = rlo - key0 - 4 * half, hi = rhi - key0 - 4 * half;
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const uint32_t bits = static_cast<uint32_t>(there >> (32 * b)) >> (4 * half);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int kk = 8 * (i / 4) + i % 4;
-          if (!(32 * b + kk >= lo && 32 * b + kk < hi && (bits >> kk & 1))) s[b][i] = kNegInf;
-        }
-      }
-    }
-    float bm0 = s[0][0], bm1 = s[1][0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) {
-      bm0 = max2(bm0, s[0][i]);
-      bm1 = max2(bm1, s[1][i]);
-    }
-    const float bm = row_max(max2(bm0, bm1));
-    const float nm = fmaxf(mx, bm * c);
-    // the maximum that weights are relative to follows only steps of more than
-    // 2^8: weights stay within [0, 256], far from any type's range, and the
-    // rescale of O is rare (without this 10 % slower)
-    if (__any(nm > mx + 8.f)) {
-      const float f = __builtin_amdgcn_exp2f(mx - (nm == kNegInf ? 0.f : nm));
-      sum *= f;
+  // A hidden key's weight is 0, but 0 times an infinite or NaN value is not:
+  // those values are added to the rows that see their key and taken out of the block.
+  auto take_infinite = [&](int buf, int key0, uint64_t there) {
+    const uint32_t vt = lds + buf * 2 * TILE + TILE;
+#pragma unroll 1
+    for (int kk = 0; kk < kTileKeys; ++kk) {
+      const bool sees = key0 + kk >= rlo && key0 + kk < rhi && (there >> kk & 1);
 #pragma unroll
       for (int m = 0; m < NB; ++m)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[m][i] *= f;
-      mx = nm;
-    }
-    const float base = mx == kNegInf ? 0.f : mx;  // (a row that has seen nothing yet)
+        for (int i = 0; i < 16; i += 2) {
+          const int d = 32 * m + 8 * (i / 4) + 4 * half + i % 4;
+          const uint32_t x = *(NNSX_LDS uint32_t*)(vt + kk * ROW + ((d / 8 ^ v_turn<DP>(kk)) << 4) + d % 8 * 2);
+          const uint32_t f = sees ? infinite<T>(x) & Bits<T>::sign : 0u;
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[b][i] = __builtin_amdgcn_exp2f(s[b][i] * c - base);
-        sum += s[b][i];
-      }
-    uint32_t inf = 0;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      u32x4 p;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) p[e] = pack2<T>(s[t / 2][8 * (t % 2) + 2 * e], s[t / 2][8 * (t % 2) + 2 * e + 1]);
-#pragma unroll
-      for (int m = 0; m < NB; ++m) {
-        u32x4 vt;
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const s16x4 x =
-              __builtin_amdgcn_ds_read_tr16_b64_v4i16((NNSX_LDS s16x4*)((vat ^ m << 6) + (16 * t + 8 * g) * ROW));
-          const u32x2 w = __builtin_bit_cast(u32x2, x);
-          vt[2 * g] = w[0];
-          vt[2 * g + 1] = w[1];
+          for (int e = 0; e < 2; ++e)
+            if (f >> (15 + 16 * e) & 1) o[m][i + e] += value_of<T>(x, e);
         }
-        if constexpr (MASKED) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            inf |= infinite<T>(vt[e]);
-            vt[e] = finite_part<T>(vt[e]);
-          }
-        }
-        o[m] = mfma16<T>(vt, p, o[m]);
-      }
     }
-    if constexpr (MASKED) {  // infinite and NaN values: to the rows that see their key (as in the stream kernel)
-      if (__any((inf & Bits<T>::sign) != 0)) {
-#pragma unroll 1
-        for (int kk = 0; kk < kTileKeys; ++kk) {
-          const bool sees = key0 + kk >= rlo && key0 + kk < rhi && (there >> kk & 1);
-#pragma unroll
-          for (int m = 0; m < NB; ++m)
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              const int d = 32 * m + 8 * (i / 4) + 4 * half + i % 4;
-              const uint32_t x = *(NNSX_LDS uint32_t*)(lds + buf * 2 * TILE + TILE + kk * ROW +
-                                                       ((d / 8 ^ v_turn<DP>(kk)) << 4) + d % 8 * 2);
-              const uint32_t f = sees ? infinite<T>(x) & Bits<T>::sign : 0u;
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                if (f >> (15 + 16 * e) & 1) o[m][i + e] += value_of<T>(x, e);
-            }
-        }
-      }
+    __syncthreads();
+    for (int i = threadIdx.x; i < TILE / 4; i += WAVES * 64) {
+      NNSX_LDS uint32_t* w = (NNSX_LDS uint32_t*)(vt + i * 4);
+      *w = finite_part<T>(*w);
     }
+    if (threadIdx.x == 0) sh_inf[buf] = 0;
+    __syncthreads();
   };
 
+  if (threadIdx.x < 2) sh_inf[threadIdx.x] = 0;
   KeyRow next = key_row(blk0);
   uint64_t there_next = __ballot(next.there);
+  auto hides = [&](int blk) {  // some row of the tile does not see some key of the block
+    return !(there_next == ~0ull && t_in_lo <= blk * kTileKeys && blk * kTileKeys + kTileKeys <= t_in_hi);
+  };
+  __syncthreads();
   if (blk0 < blk1) {
     load(next);
-    store(0);
+    store(0, hides(blk0));
   }
   next = key_row(blk0 + 1);
   for (int blk = blk0; blk < blk1; ++blk) {
@@ -859,13 +811,75 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
     if (more) load(next);
     there_next = __ballot(next.there);
     next = key_row(blk + 2);
+    if (__builtin_amdgcn_readfirstlane(sh_inf[buf])) take_infinite(buf, key0, there);
     if (key0 < whi && key0 + kTileKeys > wlo) {
-      if (there == ~0ull && __all(!live || (rlo <= key0 && key0 + kTileKeys <= rhi)))
-        block(std::false_type{}, buf, key0, there);
-      else
-        block(std::true_type{}, buf, key0, there);
+      const uint32_t kat = lds + buf * 2 * TILE + kread, vat = lds + buf * 2 * TILE + vread;
+      f32x16 s[2];
+      s[0] = s[1] = (f32x16)(0.f);
+#pragma unroll
+      for (int i = 0; i < KC; ++i)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) s[b] = mfma16<T>(*(NNSX_LDS u32x4*)((kat ^ i << 5) + b * 32 * ROW), q[i], s[b]);
+      if (!(there == ~0ull && w_in_lo <= key0 && key0 + kTileKeys <= w_in_hi)) {
+        const int lo = rlo - key0 - 4 * half, hi = rhi - key0 - 4 * half;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const uint32_t bits = static_cast<uint32_t>(there >> (32 * b)) >> (4 * half);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int kk = 8 * (i / 4) + i % 4;
+            if (!(32 * b + kk >= lo && 32 * b + kk < hi && (bits >> kk & 1))) s[b][i] = kNegInf;
+          }
+        }
+      }
+      float bm0 = s[0][0], bm1 = s[1][0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) {
+        bm0 = max2(bm0, s[0][i]);
+        bm1 = max2(bm1, s[1][i]);
+      }
+      const float nm = fmaxf(mx, row_max(max2(bm0, bm1)) * c);
+      // the maximum that weights are relative to follows only steps of more than
+      // 2^8: weights stay within [0, 256], far from any type's range, and the
+      // rescale of O is rare
+      if (__any(nm > mx + 8.f)) {
+        const float f = __builtin_amdgcn_exp2f(mx - (nm == kNegInf ? 0.f : nm));
+        sum *= f;
+#pragma unroll
+        for (int m = 0; m < NB; ++m)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[m][i] *= f;
+        mx = nm;
+      }
+      const float base = mx == kNegInf ? 0.f : mx;  // (a row that has seen nothing yet)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          s[b][i] = __builtin_amdgcn_exp2f(s[b][i] * c - base);
+          sum += s[b][i];
+        }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        u32x4 p;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e] = pack2<T>(s[t / 2][8 * (t % 2) + 2 * e], s[t / 2][8 * (t % 2) + 2 * e + 1]);
+#pragma unroll
+        for (int m = 0; m < NB; ++m) {
+          u32x4 vt;
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const s16x4 x =
+                __builtin_amdgcn_ds_read_tr16_b64_v4i16((NNSX_LDS s16x4*)((vat ^ m << 6) + (16 * t + 8 * g) * ROW));
+            const u32x2 w = __builtin_bit_cast(u32x2, x);
+            vt[2 * g] = w[0];
+            vt[2 * g + 1] = w[1];
+          }
+          o[m] = mfma16<T>(vt, p, o[m]);
+        }
+      }
     }
-    if (more) store(buf ^ 1);
+    if (more) store(buf ^ 1, hides(blk + 1));
   }
   sum = row_sum(sum);
   if (!live) return;
