@@ -265,6 +265,24 @@ __device__ __forceinline__ void key_range(const PagedAttnArgs& a, const Item& it
   if (*hi < *lo) *hi = *lo;
 }
 
+// A key's page id (as the table has it, -1 behind the item's keys) and row in the page.  Only
+// fetched here: a use of the id would wait for every load issued before it.
+struct KeyRow {
+  int id, off;
+};
+__device__ __forceinline__ KeyRow key_row(const PagedAttnArgs& a, const int* table, int key, int keys) {
+  KeyRow r{-1, 0};
+  if (key < keys) {
+    const int p = key / a.p.page;
+    r.off = key - p * a.p.page;
+    r.id = table[p];
+  }
+  return r;
+}
+__device__ __forceinline__ bool is_there(const PagedAttnArgs& a, const KeyRow& r) {
+  return static_cast<uint32_t>(r.id) < static_cast<uint32_t>(a.p.pages);
+}
+
 // workspace of a split call: per (item slot, kv head) kRows x (d floats) and kRows x (max, sum)
 __host__ __device__ __forceinline__ size_t part_floats(int rows, int d) { return static_cast<size_t>(rows) * (d + 2); }
 
@@ -360,42 +378,27 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
   uint32_t v[16][VW];
   const int vcol = NB * col;
 
-  // this lane's key (lane & 31) of a block: its rows' offsets, or not there
-  struct KeyRow {
-    int64_t k, v;
-    bool there;
-  };
-  auto key_row = [&](int blk) {
-    KeyRow r{0, 0, false};
-    const int key = blk < blk1 ? blk * kKeys + col : it.keys;
-    if (key < it.keys) {
-      const int p = key / a.p.page, off = key - p * a.p.page;
-      const int id = table[p];
-      r.there = id >= 0 && id < a.p.pages;
-      if (r.there) {
-        r.k = id * a.kp + off * a.kr;
-        r.v = id * a.vp + off * a.vr;
-      }
-    }
-    return r;
-  };
+  // this lane's key (lane & 31) of a block
+  auto row_of = [&](int blk) { return key_row(a, table, blk < blk1 ? blk * kKeys + col : it.keys, it.keys); };
   auto load_k = [&](const KeyRow& r) {
-    const E* p = kbase + r.k;
+    const bool there = is_there(a, r);
+    const E* p = kbase + r.id * a.kp + r.off * a.kr;
 #pragma unroll
     for (int s = 0; s < KC; ++s) {
       const int d = (2 * s + half) * PIECE;
       k[s] = (u32x4)(0u);
-      if (r.there && d < a.d) k[s] = *reinterpret_cast<const u32x4*>(p + d);
+      if (there && d < a.d) k[s] = *reinterpret_cast<const u32x4*>(p + d);
     }
   };
   auto load_v = [&](const KeyRow& r) {
-    const uint32_t there = static_cast<uint32_t>(__ballot(r.there)) >> (4 * half);
-    int64_t first = 0;
+    const uint32_t there = static_cast<uint32_t>(__ballot(is_there(a, r))) >> (4 * half);
+    const E* first = vbase;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int kk = 8 * (i / 4) + i % 4;
-      if (!QUAD || i % 4 == 0) first = __shfl(r.v, kk + 4 * half);
-      const E* p = vbase + first + (QUAD ? (i % 4) * a.vr : 0) + vcol;
+      if (!QUAD || i % 4 == 0)
+        first = vbase + __shfl(r.id, kk + 4 * half) * a.vp + __shfl(r.off, kk + 4 * half) * a.vr + vcol;
+      const E* p = first + (QUAD ? (i % 4) * a.vr : 0);
 #pragma unroll
       for (int w = 0; w < VW; ++w) v[i][w] = 0u;
       if ((there >> kk & 1) && vcol < a.d) {
@@ -418,7 +421,7 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
   };
 
   int blk = blk0 + wave;
-  KeyRow here = key_row(blk), then = key_row(blk + kWaves);
+  KeyRow here = row_of(blk), then = row_of(blk + kWaves);
   if (blk < blk1) {
     load_k(here);
     load_v(here);
@@ -426,7 +429,7 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
   while (blk < blk1) {
     const int next = blk + kWaves;
     const int key0 = blk * kKeys;
-    const uint32_t there = static_cast<uint32_t>(__ballot(here.there));  // (lanes 0 .. 31: the block's keys)
+    const uint32_t there = static_cast<uint32_t>(__ballot(is_there(a, here)));  // (lanes 0 .. 31: the block's keys)
     f32x16 s = (f32x16)(0.f);
     if constexpr (WIDE) {
 #pragma unroll
@@ -486,7 +489,7 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
           if (!(there >> kk & 1)) continue;
           const int key = key0 + kk;
           const bool sees = key >= rlo && key < rhi;
-          const E* p = vbase + __shfl(here.v, kk);
+          const E* p = vbase + __shfl(here.id, kk) * a.vp + __shfl(here.off, kk) * a.vr;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int d = NB * (8 * (i / 4) + 4 * half + i % 4);
@@ -533,7 +536,7 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
     }
     if (next < blk1) load_v(then);
     here = then;
-    then = key_row(next + kWaves);
+    then = row_of(next + kWaves);
     blk = next;
   }
   sum = row_sum(sum);
@@ -705,24 +708,7 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
   const float c = a.scale * kLog2e;
 
   // lane i: key i of a block
-  struct KeyRow {
-    int64_t k, v;
-    bool there;
-  };
-  auto key_row = [&](int blk) {
-    KeyRow r{0, 0, false};
-    const int key = blk < blk1 ? blk * kTileKeys + lane : it.keys;
-    if (key < it.keys) {
-      const int p = key / a.p.page, off = key - p * a.p.page;
-      const int id = table[p];
-      r.there = id >= 0 && id < a.p.pages;
-      if (r.there) {
-        r.k = id * a.kp + off * a.kr;
-        r.v = id * a.vp + off * a.vr;
-      }
-    }
-    return r;
-  };
+  auto row_of = [&](int blk) { return key_row(a, table, blk < blk1 ? blk * kTileKeys + lane : it.keys, it.keys); };
   u32x4 kr[PASSES], vr[PASSES];
   const int lrow = threadIdx.x / P, piece = threadIdx.x % P;
   // addresses in a block (K at 0, V at TILE): this lane's pieces to store, and to read
@@ -731,12 +717,13 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
   const int vrow = 4 * half + (lane & 15) / 4;
   const uint32_t vread = TILE + vrow * ROW + (((2 * (lane >> 4 & 1) + (lane & 3) / 2) ^ v_turn<DP>(vrow)) << 4) + (lane & 1) * 8;
   auto load = [&](const KeyRow& r) {
-    const uint64_t there = __ballot(r.there);
+    const uint64_t there = __ballot(is_there(a, r));
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
       const int x = i * PASS + lrow;
-      const E* kp = kbase + __shfl(r.k, x) + piece * 8;
-      const E* vp = vbase + __shfl(r.v, x) + piece * 8;
+      const int64_t id = __shfl(r.id, x), off = __shfl(r.off, x);
+      const E* kp = kbase + id * a.kp + off * a.kr + piece * 8;
+      const E* vp = vbase + id * a.vp + off * a.vr + piece * 8;
       kr[i] = vr[i] = (u32x4)(0u);
       if ((there >> x & 1) && piece * 8 < a.d) {
         kr[i] = *reinterpret_cast<const u32x4*>(kp);
@@ -792,8 +779,8 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
   };
 
   if (threadIdx.x < 2) sh_inf[threadIdx.x] = 0;
-  KeyRow next = key_row(blk0);
-  uint64_t there_next = __ballot(next.there);
+  KeyRow next = row_of(blk0);
+  uint64_t there_next = __ballot(is_there(a, next));
   auto hides = [&](int blk) {  // some row of the tile does not see some key of the block
     return !(there_next == ~0ull && t_in_lo <= blk * kTileKeys && blk * kTileKeys + kTileKeys <= t_in_hi);
   };
@@ -802,15 +789,18 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
     load(next);
     store(0, hides(blk0));
   }
-  next = key_row(blk0 + 1);
+  // Q has arrived: else its first use in the loop would wait for every load in
+  // flight there, the next block's too (vmcnt 0, the other counters free)
+  __builtin_amdgcn_s_waitcnt(0x0f70);
+  next = row_of(blk0 + 1);
   for (int blk = blk0; blk < blk1; ++blk) {
     const int buf = (blk - blk0) & 1, key0 = blk * kTileKeys;
     const uint64_t there = there_next;
     __syncthreads();  // this block is stored, the other buffer read
     const bool more = blk + 1 < blk1;
     if (more) load(next);
-    there_next = __ballot(next.there);
-    next = key_row(blk + 2);
+    there_next = __ballot(is_there(a, next));
+    next = row_of(blk + 2);
     if (__builtin_amdgcn_readfirstlane(sh_inf[buf])) take_infinite(buf, key0, there);
     if (key0 < whi && key0 + kTileKeys > wlo) {
       const uint32_t kat = lds + buf * 2 * TILE + kread, vat = lds + buf * 2 * TILE + vread;
