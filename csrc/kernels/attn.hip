@@ -114,8 +114,19 @@ __device__ __forceinline__ float value_of<F32>(uint32_t x, int) {
 __device__ __forceinline__ uint32_t interleave(uint32_t a, uint32_t b, int high) {
   return __builtin_amdgcn_perm(b, a, high ? 0x07060302u : 0x05040100u);
 }
-// max(a, b) as one instruction (fmaxf first quiets both operands); a NaN loses
-__device__ __forceinline__ float max2(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, __builtin_huge_valf()); }
+// max(a, b) as one instruction, the middle of a, b and infinity (fmaxf first quiets both
+// operands, and so would this if the compiler knew the constant); a NaN loses
+__device__ __forceinline__ float max2(float a, float b) {
+  float inf;
+  asm("s_mov_b32 %0, 0x7f800000" : "=s"(inf));
+  return __builtin_amdgcn_fmed3f(a, b, inf);
+}
+// max(a, b, c) likewise, of results that no matrix instruction wrote (the compiler keeps no distance for asm)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
 // over the two lanes of a row, 32 apart
 __device__ __forceinline__ float row_max(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -279,6 +290,29 @@ __device__ __forceinline__ KeyRow key_row(const PagedAttnArgs& a, const int* tab
   }
   return r;
 }
+// The same for keys that go on by STEP: divides once
+template <int STEP>
+struct KeyWalk {
+  int key, p, off, dp, doff;
+  __device__ __forceinline__ KeyWalk(const PagedAttnArgs& a, int first) : key(first) {
+    p = key / a.p.page;
+    off = key - p * a.p.page;
+    dp = STEP / a.p.page;
+    doff = STEP - dp * a.p.page;
+  }
+  __device__ __forceinline__ KeyRow next(const PagedAttnArgs& a, const int* table, int keys) {
+    KeyRow r{-1, off};
+    if (key < keys) r.id = table[p];
+    key = min(key + STEP, keys);
+    p += dp;
+    off += doff;
+    if (off >= a.p.page) {
+      off -= a.p.page;
+      ++p;
+    }
+    return r;
+  }
+};
 __device__ __forceinline__ bool is_there(const PagedAttnArgs& a, const KeyRow& r) {
   return static_cast<uint32_t>(r.id) < static_cast<uint32_t>(a.p.pages);
 }
@@ -708,26 +742,39 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
   const float c = a.scale * kLog2e;
 
   // lane i: key i of a block
-  auto row_of = [&](int blk) { return key_row(a, table, blk < blk1 ? blk * kTileKeys + lane : it.keys, it.keys); };
+  const int keys1 = min(it.keys, blk1 * kTileKeys);
+  KeyWalk<kTileKeys> walk(a, min(blk0 * kTileKeys + lane, keys1));
   u32x4 kr[PASSES], vr[PASSES];
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) kr[i] = vr[i] = (u32x4)(0u);
   const int lrow = threadIdx.x / P, piece = threadIdx.x % P;
+  const bool piece_live = piece * 8 < a.d;  // (else the registers stay 0)
+  const E *kp = kbase + piece * 8, *vp = vbase + piece * 8;
+  const bool alike = a.kp == a.vp && a.kr == a.vr;
   // addresses in a block (K at 0, V at TILE): this lane's pieces to store, and to read
   // (passes are a multiple of 16 rows or, for 256 columns, 8: each has its own turn)
   const uint32_t kread = col * ROW + ((half ^ k_turn<DP>(col)) << 4);
   const int vrow = 4 * half + (lane & 15) / 4;
   const uint32_t vread = TILE + vrow * ROW + (((2 * (lane >> 4 & 1) + (lane & 3) / 2) ^ v_turn<DP>(vrow)) << 4) + (lane & 1) * 8;
-  auto load = [&](const KeyRow& r) {
-    const uint64_t there = __ballot(is_there(a, r));
+  // A key that is not there is read from the cache's first row: a hidden one of the block
+  auto load = [&](const KeyRow& r, uint64_t there) {
+    if (there == 0) return;
+    const bool ok = is_there(a, r);
+    const int64_t id = ok ? r.id : 0, off = ok ? r.off : 0;
+    int64_t xk[PASSES], xv[PASSES];
+    const int64_t ko = id * a.kp + off * a.kr;
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      const int x = i * PASS + lrow;
-      const int64_t id = __shfl(r.id, x), off = __shfl(r.off, x);
-      const E* kp = kbase + id * a.kp + off * a.kr + piece * 8;
-      const E* vp = vbase + id * a.vp + off * a.vr + piece * 8;
-      kr[i] = vr[i] = (u32x4)(0u);
-      if ((there >> x & 1) && piece * 8 < a.d) {
-        kr[i] = *reinterpret_cast<const u32x4*>(kp);
-        vr[i] = *reinterpret_cast<const u32x4*>(vp);
+    for (int i = 0; i < PASSES; ++i) xk[i] = xv[i] = __shfl(ko, i * PASS + lrow);
+    if (!alike) {
+      const int64_t vo = id * a.vp + off * a.vr;
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i) xv[i] = __shfl(vo, i * PASS + lrow);
+    }
+    if (piece_live) {
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i) {
+        kr[i] = *reinterpret_cast<const u32x4*>(kp + xk[i]);
+        vr[i] = *reinterpret_cast<const u32x4*>(vp + xv[i]);
       }
     }
   };
@@ -779,28 +826,28 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
   };
 
   if (threadIdx.x < 2) sh_inf[threadIdx.x] = 0;
-  KeyRow next = row_of(blk0);
+  KeyRow next = walk.next(a, table, keys1);
   uint64_t there_next = __ballot(is_there(a, next));
   auto hides = [&](int blk) {  // some row of the tile does not see some key of the block
     return !(there_next == ~0ull && t_in_lo <= blk * kTileKeys && blk * kTileKeys + kTileKeys <= t_in_hi);
   };
   __syncthreads();
   if (blk0 < blk1) {
-    load(next);
+    load(next, there_next);
     store(0, hides(blk0));
   }
   // Q has arrived: else its first use in the loop would wait for every load in
   // flight there, the next block's too (vmcnt 0, the other counters free)
   __builtin_amdgcn_s_waitcnt(0x0f70);
-  next = row_of(blk0 + 1);
+  next = walk.next(a, table, keys1);
   for (int blk = blk0; blk < blk1; ++blk) {
     const int buf = (blk - blk0) & 1, key0 = blk * kTileKeys;
     const uint64_t there = there_next;
     __syncthreads();  // this block is stored, the other buffer read
     const bool more = blk + 1 < blk1;
-    if (more) load(next);
     there_next = __ballot(is_there(a, next));
-    next = row_of(blk + 2);
+    if (more) load(next, there_next);
+    next = walk.next(a, table, keys1);
     if (__builtin_amdgcn_readfirstlane(sh_inf[buf])) take_infinite(buf, key0, there);
     if (key0 < whi && key0 + kTileKeys > wlo) {
       const uint32_t kat = lds + buf * 2 * TILE + kread, vat = lds + buf * 2 * TILE + vread;
@@ -822,13 +869,11 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
           }
         }
       }
-      float bm0 = s[0][0], bm1 = s[1][0];
+      float bm = max2(s[0][0], s[1][0]);
 #pragma unroll
-      for (int i = 1; i < 16; ++i) {
-        bm0 = max2(bm0, s[0][i]);
-        bm1 = max2(bm1, s[1][i]);
-      }
-      const float nm = fmaxf(mx, row_max(max2(bm0, bm1)) * c);
+      for (int i = 1; i < 15; i += 2) bm = max3(bm, max2(s[0][i], s[1][i]), max2(s[0][i + 1], s[1][i + 1]));
+      bm = max2(bm, max2(s[0][15], s[1][15]));
+      const float nm = fmaxf(mx, row_max(bm) * c);
       // the maximum that weights are relative to follows only steps of more than
       // 2^8: weights stay within [0, 256], far from any type's range, and the
       // rescale of O is rare
