@@ -116,10 +116,11 @@ __device__ __forceinline__ uint32_t interleave(uint32_t a, uint32_t b, int high)
 }
 // max(a, b) as one instruction, the middle of a, b and infinity (fmaxf first quiets both
 // operands, and so would this if the compiler knew the constant); a NaN loses
-__device__ __forceinline__ float max2(float a, float b) {
+__device__ __forceinline__ float max2(float a, float b, float inf) { return __builtin_amdgcn_fmed3f(a, b, inf); }
+__device__ __forceinline__ float opaque_infinity() {
   float inf;
-  asm("s_mov_b32 %0, 0x7f800000" : "=s"(inf));
-  return __builtin_amdgcn_fmed3f(a, b, inf);
+  asm volatile("s_mov_b32 %0, 0x7f800000" : "=s"(inf));
+  return inf;
 }
 // max(a, b, c) likewise, of results that no matrix instruction wrote (the compiler keeps no distance for asm)
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -128,9 +129,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 // over the two lanes of a row, 32 apart
-__device__ __forceinline__ float row_max(float x) {
+__device__ __forceinline__ float row_max(float x, float inf) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return max2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  return max2(__uint_as_float(r[0]), __uint_as_float(r[1]), inf);
 }
 __device__ __forceinline__ float row_sum(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -290,29 +291,6 @@ __device__ __forceinline__ KeyRow key_row(const PagedAttnArgs& a, const int* tab
   }
   return r;
 }
-// The same for keys that go on by STEP: divides once
-template <int STEP>
-struct KeyWalk {
-  int key, p, off, dp, doff;
-  __device__ __forceinline__ KeyWalk(const PagedAttnArgs& a, int first) : key(first) {
-    p = key / a.p.page;
-    off = key - p * a.p.page;
-    dp = STEP / a.p.page;
-    doff = STEP - dp * a.p.page;
-  }
-  __device__ __forceinline__ KeyRow next(const PagedAttnArgs& a, const int* table, int keys) {
-    KeyRow r{-1, off};
-    if (key < keys) r.id = table[p];
-    key = min(key + STEP, keys);
-    p += dp;
-    off += doff;
-    if (off >= a.p.page) {
-      off -= a.p.page;
-      ++p;
-    }
-    return r;
-  }
-};
 __device__ __forceinline__ bool is_there(const PagedAttnArgs& a, const KeyRow& r) {
   return static_cast<uint32_t>(r.id) < static_cast<uint32_t>(a.p.pages);
 }
@@ -404,7 +382,7 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
 #pragma unroll
   for (int m = 0; m < NB; ++m) o[m] = (f32x16)(0.f);
   float mx = kNegInf, sum = 0.f;
-  const float c = a.scale * kLog2e;
+  const float c = a.scale * kLog2e, inf = opaque_infinity();
 
   u32x4 k[KC];
   // V: 16 rows a lane half, NB neighbouring columns: NB / 2 words (16 bit) or NB (32 bit)
@@ -489,8 +467,8 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
     }
     float bm = s[0];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) bm = max2(bm, s[i]);
-    bm = row_max(bm);
+    for (int i = 1; i < 16; ++i) bm = max2(bm, s[i], inf);
+    bm = row_max(bm, inf);
     const float nm = fmaxf(mx, bm * c);
     const float base = nm == kNegInf ? 0.f : nm;  // (a row that has seen nothing yet)
     if (__any(nm > mx)) {
@@ -512,12 +490,12 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
     // is 0 there, but 0 times an infinite or NaN value is not: in such a block
     // those values are taken out of V and added to the rows that see their key.
     if (!full) {
-      uint32_t inf = 0;
+      uint32_t odd = 0;
 #pragma unroll
       for (int i = 0; i < 16; ++i)
 #pragma unroll
-        for (int w = 0; w < VW; ++w) inf |= infinite<T>(v[i][w]);
-      if (__any((inf & Bits<T>::sign) != 0)) {
+        for (int w = 0; w < VW; ++w) odd |= infinite<T>(v[i][w]);
+      if (__any((odd & Bits<T>::sign) != 0)) {
 #pragma unroll 1
         for (int kk = 0; kk < kKeys; ++kk) {
           if (!(there >> kk & 1)) continue;
@@ -648,44 +626,40 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
 
 // -------------------------------------------------------------- tile kernel ----
 // Many rows of one sequence: a workgroup of WAVES waves takes 32 rows each and
-// all walk over the same key blocks of 64, staged through LDS in two buffers:
-// the next block's rows are loaded to registers before the current one is
-// worked on and stored after it, with one barrier a block.  K rows are read as
-// 16-byte pieces; V^T comes out of the row-major tile through the transposing
-// LDS read (ds_read_b64_tr_b16: 16 lanes read 4 keys x 16 columns and each gets
-// one column's 4 keys).  Pieces of a row are stored at piece ^ f(row), with f
-// such that the 16 lanes of a read (K: 16 rows, one piece; V: 4 rows, 4 pieces) touch every bank once.
+// all walk over the same key blocks of 64, staged through LDS in two buffers: a
+// block's rows are loaded straight to LDS while the one before it is worked on,
+// with one barrier a block.  K rows are read as 16-byte pieces; V^T comes out of
+// the row-major tile through the transposing LDS read (ds_read_b64_tr_b16: 16
+// lanes read 4 keys x 16 columns and each gets one column's 4 keys).  Pieces of
+// a row are stored at piece ^ turn(row), such that the 16 lanes of a read (K:
+// 16 rows, one piece; V: 4 rows, 4 pieces) touch every bank once.
 constexpr int kTileKeys = 64;
 
-// What piece numbers of a row are combined with (exclusive or).  A row of 128
-// bytes shares the 256 bytes that the banks hold with its neighbour.
+// A row of 128 bytes shares the 256 bytes that the banks hold with its neighbour.
 template <int DP>
-__device__ __forceinline__ int k_turn(int row) {
-  return DP >= 128 ? row & 15 : row >> 1 & 7;
-}
-template <int DP>
-__device__ __forceinline__ int v_turn(int row) {
-  return DP >= 128 ? (row & 3) << 2 : (row >> 1 & 1) << 2;
+__device__ __forceinline__ int turn(int row) {
+  return (DP >= 128 ? row & 3 : row >> 1 & 1) << 2 | (row >> 2 & 3);
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 #define NNSX_LDS __attribute__((address_space(3)))
+#define NNSX_GLOBAL __attribute__((address_space(1)))
 
-template <typename T, int DP, int WAVES>
+template <typename T, int DP, int WAVES, bool ONE_PAGE>
 __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile(PagedAttnArgs a) {
   using E = uint16_t;
   constexpr int ROWS = WAVES * 32, NB = DP / 32, KC = DP / 16, P = DP / 8;
-  constexpr int PASS = WAVES * 64 / P;                 // rows of a tile that the workgroup loads at once
+  constexpr int PASS = WAVES * 64 / P;       // rows of a block that the workgroup loads at once,
+  constexpr int RUN = 64 / P;                // a wave's of them (1 KiB)
   constexpr int PASSES = kTileKeys / PASS;
-  static_assert(PASS * PASSES == kTileKeys && 64 % P == 0 && PASS >= 1, "tile");
+  static_assert(PASS * PASSES == kTileKeys && RUN * P == 64 && PASSES <= 64, "tile");
   __shared__ int64_t sh_scan[WAVES];
   __shared__ int sh_found[kFound];
-  // K and V of two blocks; rows are aligned to their size, so that pieces of a row are reached by exclusive or
+  // K and V of two blocks, an array each: the compiler keeps them apart, so that a read of one
+  // does not wait for the loads into another.  Rows are aligned to their size, so that pieces
+  // of a row are reached by exclusive or.
   constexpr int ROW = DP * 2, TILE = kTileKeys * ROW;
-  __shared__ __attribute__((aligned(1024))) char sh_kv[4 * TILE];
-  __shared__ int sh_inf[2];
-  const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((NNSX_LDS char*)sh_kv));
-
+  __shared__ __attribute__((aligned(1024))) char sh_k0[TILE], sh_k1[TILE], sh_v0[TILE], sh_v1[TILE];
   const int head = static_cast<int>(blockIdx.x % a.hkv);
   const int slot = static_cast<int>(blockIdx.x / a.hkv);
   const Item it = find_item<ROWS, kTileKeys, false>(a, slot, sh_scan, sh_found);
@@ -697,9 +671,9 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
   const int row = it.tile * ROWS + wave * 32 + col;
   const bool live = row < rows;
   const int tok = row / a.group, gh = row - tok * a.group;
-  // keys that this lane's row sees; that some (lo, hi) and that every row (in_lo,
-  // in_hi) of the tile (t) and of the wave (w) sees
-  int rlo, rhi, tlo, thi, t_in_lo, t_in_hi, wlo = 0, whi = 0, w_in_lo = 0, w_in_hi = 0, x;
+  // keys that this lane's row sees; that some row of the tile sees; that every
+  // row of the tile (t_in) and of the wave (w_in) sees
+  int rlo, rhi, tlo, thi, t_in_lo, t_in_hi, w_in_lo = 0, w_in_hi = 0x7fffffff, x;
   key_range(a, it, tok, tok, &rlo, &rhi);
   if (!live) rhi = rlo = 0;
   {
@@ -708,8 +682,7 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
     key_range(a, it, f / a.group, f / a.group, &x, &t_in_hi);
     key_range(a, it, l / a.group, l / a.group, &t_in_lo, &x);
     const int wf = f + wave * 32, wl = min(wf + 32, rows) - 1;
-    if (wf < rows) {
-      key_range(a, it, wf / a.group, wl / a.group, &wlo, &whi);
+    if (wf < rows) {  // (else nothing of the wave matters)
       key_range(a, it, wf / a.group, wf / a.group, &x, &w_in_hi);
       key_range(a, it, wl / a.group, wl / a.group, &w_in_lo, &x);
     }
@@ -739,68 +712,92 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
 #pragma unroll
   for (int m = 0; m < NB; ++m) o[m] = (f32x16)(0.f);
   float mx = kNegInf, sum = 0.f;
-  const float c = a.scale * kLog2e;
+  const float c = a.scale * kLog2e, inf = opaque_infinity();
 
-  // lane i: key i of a block
+  if (a.p.pages == 0) blk1 = blk0;
   const int keys1 = min(it.keys, blk1 * kTileKeys);
-  KeyWalk<kTileKeys> walk(a, min(blk0 * kTileKeys + lane, keys1));
-  u32x4 kr[PASSES], vr[PASSES];
+  // Does the table name a page that is not there, among the item's?  (Hardly ever: then blocks are looked over one by one.)
+  bool missing = false;
+  if (blk0 < blk1) {
+    for (int p = blk0 * kTileKeys / a.p.page + threadIdx.x; p <= (keys1 - 1) / a.p.page; p += WAVES * 64)
+      missing |= static_cast<uint32_t>(table[p]) >= static_cast<uint32_t>(a.p.pages);
+    missing = __syncthreads_or(missing);
+  }
+  auto there_of = [&](int blk) {
+    const int key = blk * kTileKeys + lane;
+    return __ballot(key >= keys1 || static_cast<uint32_t>(table[key / a.p.page]) < static_cast<uint32_t>(a.p.pages));
+  };
+
+  // This wave's loads: in every pass the RUN rows from i PASS + wave RUN on; lane: slot lane % P
+  // of LDS row lane / P, which holds piece (lane % P) ^ turn.  A row behind the last key or of a
+  // page that is not there is some other row of the cache: its key is hidden from every row of the tile.
+  const int lrow = lane / P;
+  const int piece[2] = {(lane % P) ^ turn<DP>(wave * RUN + lrow), (lane % P) ^ turn<DP>(PASS + wave * RUN + lrow)};
+  auto piece_of = [&](int i) { return piece[i % 2]; };  // (the turn repeats every 16 rows, two passes at most)
+  static_assert(PASS % 16 == 0 || 2 * PASS % 16 == 0, "tile");
+  const int last_page = blk0 < blk1 ? (keys1 - 1) / a.p.page : 0;
+  // ONE_PAGE: the rows of a run share a page; lane i looks after pass i.  Else every lane after its own rows.
+  constexpr int WALKS = ONE_PAGE ? 1 : PASSES;
+  int walk_p[WALKS], walk_off[WALKS], id[WALKS], off[WALKS];
+  const int dp = kTileKeys / a.p.page, doff = kTileKeys - dp * a.p.page;
 #pragma unroll
-  for (int i = 0; i < PASSES; ++i) kr[i] = vr[i] = (u32x4)(0u);
-  const int lrow = threadIdx.x / P, piece = threadIdx.x % P;
-  const bool piece_live = piece * 8 < a.d;  // (else the registers stay 0)
-  const E *kp = kbase + piece * 8, *vp = vbase + piece * 8;
-  const bool alike = a.kp == a.vp && a.kr == a.vr;
-  // addresses in a block (K at 0, V at TILE): this lane's pieces to store, and to read
-  // (passes are a multiple of 16 rows or, for 256 columns, 8: each has its own turn)
-  const uint32_t kread = col * ROW + ((half ^ k_turn<DP>(col)) << 4);
-  const int vrow = 4 * half + (lane & 15) / 4;
-  const uint32_t vread = TILE + vrow * ROW + (((2 * (lane >> 4 & 1) + (lane & 3) / 2) ^ v_turn<DP>(vrow)) << 4) + (lane & 1) * 8;
-  // A key that is not there is read from the cache's first row: a hidden one of the block
-  auto load = [&](const KeyRow& r, uint64_t there) {
-    if (there == 0) return;
-    const bool ok = is_there(a, r);
-    const int64_t id = ok ? r.id : 0, off = ok ? r.off : 0;
-    int64_t xk[PASSES], xv[PASSES];
-    const int64_t ko = id * a.kp + off * a.kr;
+  for (int i = 0; i < WALKS; ++i) {
+    const int key = blk0 * kTileKeys + wave * RUN + (ONE_PAGE ? lane % PASSES * PASS : i * PASS + lrow);
+    walk_p[i] = key / a.p.page;
+    walk_off[i] = key - walk_p[i] * a.p.page;
+  }
+  auto fetch = [&]() __attribute__((always_inline)) {  // page ids of the next block
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) xk[i] = xv[i] = __shfl(ko, i * PASS + lrow);
-    if (!alike) {
-      const int64_t vo = id * a.vp + off * a.vr;
-#pragma unroll
-      for (int i = 0; i < PASSES; ++i) xv[i] = __shfl(vo, i * PASS + lrow);
-    }
-    if (piece_live) {
-#pragma unroll
-      for (int i = 0; i < PASSES; ++i) {
-        kr[i] = *reinterpret_cast<const u32x4*>(kp + xk[i]);
-        vr[i] = *reinterpret_cast<const u32x4*>(vp + xv[i]);
+    for (int i = 0; i < WALKS; ++i) {
+      id[i] = table[min(walk_p[i], last_page)];
+      off[i] = walk_off[i];
+      walk_p[i] += dp;
+      walk_off[i] += doff;
+      if (walk_off[i] >= a.p.page) {
+        walk_off[i] -= a.p.page;
+        ++walk_p[i];
       }
     }
   };
-  // check: a key of the block is hidden from some row of the tile; then infinite and NaN values are flagged
-  auto store = [&](int buf, bool check) {
-    if (check) {
-      uint32_t inf = 0;
+  const uint32_t page_k = static_cast<uint32_t>(a.kp) * 2, row_k = static_cast<uint32_t>(a.kr) * 2;  // bytes
+  const uint32_t page_v = static_cast<uint32_t>(a.vp) * 2, row_v = static_cast<uint32_t>(a.vr) * 2;
+  uint64_t from_k[WALKS], from_v[WALKS];
+  auto locate = [&]() __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < PASSES; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) inf |= infinite<T>(vr[i][e]);
-      if (inf & Bits<T>::sign) sh_inf[buf] = 1;
-    }
-#pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      const int x = i * PASS + lrow;
-      const uint32_t at = lds + buf * 2 * TILE + x * ROW;
-      *(NNSX_LDS u32x4*)(at + ((piece ^ k_turn<DP>(x)) << 4)) = kr[i];
-      *(NNSX_LDS u32x4*)(at + TILE + ((piece ^ v_turn<DP>(x)) << 4)) = vr[i];
+    for (int i = 0; i < WALKS; ++i) {
+      const uint32_t x = static_cast<uint32_t>(id[i]) < static_cast<uint32_t>(a.p.pages) ? id[i] : 0;
+      from_k[i] = reinterpret_cast<uint64_t>(kbase) + static_cast<uint64_t>(x) * page_k + static_cast<uint64_t>(static_cast<uint32_t>(off[i])) * row_k;
+      from_v[i] = reinterpret_cast<uint64_t>(vbase) + static_cast<uint64_t>(x) * page_v + static_cast<uint64_t>(static_cast<uint32_t>(off[i])) * row_v;
     }
   };
+  const uint32_t lane_k = ONE_PAGE ? lrow * row_k : 0, lane_v = ONE_PAGE ? lrow * row_v : 0;
+  auto load = [&](char* to, const uint64_t* from, uint32_t lane_off) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      uint64_t x = from[ONE_PAGE ? 0 : i];
+      if constexpr (ONE_PAGE)
+        x = static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(x >> 32), i)) << 32 |
+            static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(x), i));
+      const char* p = reinterpret_cast<const char*>(x) + (lane_off + piece_of(i) * 16);
+      if (piece_of(i) * 8 < a.d)  // (else the piece stays 0)
+        __builtin_amdgcn_global_load_lds((const NNSX_GLOBAL void*)p, (NNSX_LDS void*)(to + (i * WAVES + wave) * 1024), 16, 0, 0);
+    }
+  };
+  // Addresses to read in a buffer
+  const uint32_t kread = col * ROW + ((half ^ turn<DP>(col)) << 4);
+  const int vrow = 4 * half + (lane & 15) / 4, vx = 2 * (lane >> 4 & 1) + (lane & 3) / 2;
+  uint32_t vread[2];
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+    vread[g] = (vrow + 8 * g) * ROW + ((vx ^ turn<DP>(vrow + 8 * g)) << 4) + (lane & 1) * 8;
 
-  // A hidden key's weight is 0, but 0 times an infinite or NaN value is not:
-  // those values are added to the rows that see their key and taken out of the block.
-  auto take_infinite = [&](int buf, int key0, uint64_t there) {
-    const uint32_t vt = lds + buf * 2 * TILE + TILE;
+  // A hidden key's weight is 0, but 0 times an infinite or NaN value is not: in
+  // a block that hides a key from some row, those values are added to the rows
+  // that see their key and taken out of the block.
+  auto take_infinite = [&](char* v, int key0, uint64_t there) __attribute__((always_inline)) {
+    uint32_t odd = 0;
+    for (int i = threadIdx.x; i < TILE / 4; i += WAVES * 64) odd |= infinite<T>(reinterpret_cast<uint32_t*>(v)[i]);
+    if (!__syncthreads_or((odd & Bits<T>::sign) != 0)) return;
 #pragma unroll 1
     for (int kk = 0; kk < kTileKeys; ++kk) {
       const bool sees = key0 + kk >= rlo && key0 + kk < rhi && (there >> kk & 1);
@@ -809,7 +806,7 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
           const int d = 32 * m + 8 * (i / 4) + 4 * half + i % 4;
-          const uint32_t x = *(NNSX_LDS uint32_t*)(vt + kk * ROW + ((d / 8 ^ v_turn<DP>(kk)) << 4) + d % 8 * 2);
+          const uint32_t x = *reinterpret_cast<const uint32_t*>(v + kk * ROW + ((d / 8 ^ turn<DP>(kk)) << 4) + d % 8 * 2);
           const uint32_t f = sees ? infinite<T>(x) & Bits<T>::sign : 0u;
 #pragma unroll
           for (int e = 0; e < 2; ++e)
@@ -818,104 +815,127 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
     }
     __syncthreads();
     for (int i = threadIdx.x; i < TILE / 4; i += WAVES * 64) {
-      NNSX_LDS uint32_t* w = (NNSX_LDS uint32_t*)(vt + i * 4);
+      uint32_t* w = reinterpret_cast<uint32_t*>(v) + i;
       *w = finite_part<T>(*w);
     }
-    if (threadIdx.x == 0) sh_inf[buf] = 0;
     __syncthreads();
   };
 
-  if (threadIdx.x < 2) sh_inf[threadIdx.x] = 0;
-  KeyRow next = walk.next(a, table, keys1);
-  uint64_t there_next = __ballot(is_there(a, next));
-  auto hides = [&](int blk) {  // some row of the tile does not see some key of the block
-    return !(there_next == ~0ull && t_in_lo <= blk * kTileKeys && blk * kTileKeys + kTileKeys <= t_in_hi);
-  };
-  __syncthreads();
-  if (blk0 < blk1) {
-    load(next, there_next);
-    store(0, hides(blk0));
-  }
-  // Q has arrived: else its first use in the loop would wait for every load in
-  // flight there, the next block's too (vmcnt 0, the other counters free)
-  __builtin_amdgcn_s_waitcnt(0x0f70);
-  next = walk.next(a, table, keys1);
-  for (int blk = blk0; blk < blk1; ++blk) {
-    const int buf = (blk - blk0) & 1, key0 = blk * kTileKeys;
-    const uint64_t there = there_next;
-    __syncthreads();  // this block is stored, the other buffer read
-    const bool more = blk + 1 < blk1;
-    there_next = __ballot(is_there(a, next));
-    if (more) load(next, there_next);
-    next = walk.next(a, table, keys1);
-    if (__builtin_amdgcn_readfirstlane(sh_inf[buf])) take_infinite(buf, key0, there);
-    if (key0 < whi && key0 + kTileKeys > wlo) {
-      const uint32_t kat = lds + buf * 2 * TILE + kread, vat = lds + buf * 2 * TILE + vread;
-      f32x16 s[2];
-      s[0] = s[1] = (f32x16)(0.f);
+  // Block blk from k and v, while the next one is loaded to kn and vn
+  auto step = [&](char* k, char* v, char* kn, char* vn, int blk) __attribute__((always_inline)) {
+    const int key0 = blk * kTileKeys;
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // this wave's loads of the block have arrived (vmcnt 0)
+    __syncthreads();                     // every wave's have, and the other buffers are read
+    locate();
+    load(kn, from_k, lane_k);
+    f32x16 s[2];
+    constexpr int NK = 2 * KC, AHEAD = 6;  // matrix instructions of the scores, pieces of K read ahead
+    u32x4 kf[AHEAD];
+    auto read_k = [&](int j) __attribute__((always_inline)) {
+      kf[j % AHEAD] = *reinterpret_cast<const u32x4*>(k + ((kread ^ (j / 2) << 5) + j % 2 * 32 * ROW));
+    };
 #pragma unroll
-      for (int i = 0; i < KC; ++i)
+    for (int j = 0; j < AHEAD; ++j) read_k(j);
+    s[0] = s[1] = (f32x16)(0.f);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int b = 0; b < 2; ++b) s[b] = mfma16<T>(*(NNSX_LDS u32x4*)((kat ^ i << 5) + b * 32 * ROW), q[i], s[b]);
-      if (!(there == ~0ull && w_in_lo <= key0 && key0 + kTileKeys <= w_in_hi)) {
-        const int lo = rlo - key0 - 4 * half, hi = rhi - key0 - 4 * half;
+    for (int j = 0; j < NK; ++j) {
+      s[j % 2] = mfma16<T>(kf[j % AHEAD], q[j / 2], s[j % 2]);
+      if (j + AHEAD < NK) read_k(j + AHEAD);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    uint64_t there = ~0ull;
+    if (missing) there = there_of(blk);
+    load(vn, from_v, lane_v);
+    fetch();
+    if (there != ~0ull || key0 < w_in_lo || key0 + kTileKeys > w_in_hi) {
+      const int lo = rlo - key0 - 4 * half, hi = rhi - key0 - 4 * half;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const uint32_t bits = static_cast<uint32_t>(there >> (32 * b)) >> (4 * half);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int kk = 8 * (i / 4) + i % 4;
-            if (!(32 * b + kk >= lo && 32 * b + kk < hi && (bits >> kk & 1))) s[b][i] = kNegInf;
-          }
-        }
-      }
-      float bm = max2(s[0][0], s[1][0]);
-#pragma unroll
-      for (int i = 1; i < 15; i += 2) bm = max3(bm, max2(s[0][i], s[1][i]), max2(s[0][i + 1], s[1][i + 1]));
-      bm = max2(bm, max2(s[0][15], s[1][15]));
-      const float nm = fmaxf(mx, row_max(bm) * c);
-      // the maximum that weights are relative to follows only steps of more than
-      // 2^8: weights stay within [0, 256], far from any type's range, and the
-      // rescale of O is rare
-      if (__any(nm > mx + 8.f)) {
-        const float f = __builtin_amdgcn_exp2f(mx - (nm == kNegInf ? 0.f : nm));
-        sum *= f;
-#pragma unroll
-        for (int m = 0; m < NB; ++m)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[m][i] *= f;
-        mx = nm;
-      }
-      const float base = mx == kNegInf ? 0.f : mx;  // (a row that has seen nothing yet)
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < 2; ++b) {
+        const uint32_t bits = static_cast<uint32_t>(there >> (32 * b)) >> (4 * half);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          s[b][i] = __builtin_amdgcn_exp2f(s[b][i] * c - base);
-          sum += s[b][i];
-        }
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        u32x4 p;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) p[e] = pack2<T>(s[t / 2][8 * (t % 2) + 2 * e], s[t / 2][8 * (t % 2) + 2 * e + 1]);
-#pragma unroll
-        for (int m = 0; m < NB; ++m) {
-          u32x4 vt;
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const s16x4 x =
-                __builtin_amdgcn_ds_read_tr16_b64_v4i16((NNSX_LDS s16x4*)((vat ^ m << 6) + (16 * t + 8 * g) * ROW));
-            const u32x2 w = __builtin_bit_cast(u32x2, x);
-            vt[2 * g] = w[0];
-            vt[2 * g + 1] = w[1];
-          }
-          o[m] = mfma16<T>(vt, p, o[m]);
+          const int kk = 8 * (i / 4) + i % 4;
+          if (!(32 * b + kk >= lo && 32 * b + kk < hi && (bits >> kk & 1))) s[b][i] = kNegInf;
         }
       }
     }
-    if (more) store(buf ^ 1, hides(blk + 1));
+    float bm = max2(s[0][0], s[1][0], inf);
+#pragma unroll
+    for (int i = 1; i < 15; i += 2) bm = max3(bm, max2(s[0][i], s[1][i], inf), max2(s[0][i + 1], s[1][i + 1], inf));
+    const float nm = fmaxf(mx, row_max(max2(bm, max2(s[0][15], s[1][15], inf), inf), inf) * c);
+    // the maximum that weights are relative to follows only steps of more than
+    // 2^8: weights stay within [0, 256], far from any type's range, and the
+    // rescale of O is rare
+    if (__any(nm > mx + 8.f)) {
+      const float f = __builtin_amdgcn_exp2f(mx - (nm == kNegInf ? 0.f : nm));
+      sum *= f;
+#pragma unroll
+      for (int m = 0; m < NB; ++m)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[m][i] *= f;
+      mx = nm;
+    }
+    if (there != ~0ull || key0 < t_in_lo || key0 + kTileKeys > t_in_hi) take_infinite(v, key0, there);
+    const float base = mx == kNegInf ? 0.f : mx;  // (a row that has seen nothing yet)
+    u32x4 p[4];
+    auto weigh = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float w[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          w[h] = __builtin_amdgcn_exp2f(s[t / 2][8 * (t % 2) + 2 * e + h] * c - base);
+          sum += w[h];
+        }
+        p[t][e] = pack2<T>(w[0], w[1]);
+      }
+    };
+    constexpr int NV = 4 * NB, VAHEAD = 4;  // matrix instructions of the values, pieces of V^T read ahead
+    u32x4 vf[VAHEAD];
+    auto read_v = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (NNSX_LDS s16x4*)(v + ((vread[g] ^ (j % NB) << 6) + j / NB * 16 * ROW))));
+        vf[j % VAHEAD][2 * g] = x[0];
+        vf[j % VAHEAD][2 * g + 1] = x[1];
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < VAHEAD; ++j) read_v(j);
+    weigh(0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int m = 0; m < NB; ++m) {
+        const int j = t * NB + m;
+        o[m] = mfma16<T>(vf[j % VAHEAD], p[t], o[m]);
+        if (j + VAHEAD < NV) read_v(j + VAHEAD);
+      }
+      if (t < 3) weigh(t + 1);  // (while the matrix unit works)
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  // (columns from d on are never loaded: they stay 0)
+  for (int i = threadIdx.x; i < TILE / 16; i += WAVES * 64)
+    for (char* x : {sh_k0, sh_k1, sh_v0, sh_v1}) reinterpret_cast<u32x4*>(x)[i] = (u32x4)(0u);
+  if (blk0 < blk1) {
+    fetch();
+    __syncthreads();
+    locate();
+    load(sh_k0, from_k, lane_k);
+    load(sh_v0, from_v, lane_v);
+    fetch();
   }
+  for (int blk = blk0; blk < blk1; blk += 2) {
+    step(sh_k0, sh_v0, sh_k1, sh_v1, blk);
+    if (blk + 1 >= blk1) break;
+    step(sh_k1, sh_v1, sh_k0, sh_v0, blk + 1);
+  }
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // (the last block loaded one too many)
   sum = row_sum(sum);
   if (!live) return;
 
@@ -1047,6 +1067,14 @@ void launch_stream(const PagedAttnArgs& a, hipStream_t s) {
     paged_attn_stream<T, 256, QUAD><<<grid, kThreads, 0, s>>>(a);
 }
 
+template <typename T, int DP, int WAVES>
+void launch_tile(const PagedAttnArgs& a, unsigned grid, hipStream_t s) {
+  if (a.p.page % (512 / DP) == 0)  // (the keys of 1 KiB)
+    paged_attn_tile<T, DP, WAVES, true><<<grid, WAVES * 64, 0, s>>>(a);
+  else
+    paged_attn_tile<T, DP, WAVES, false><<<grid, WAVES * 64, 0, s>>>(a);
+}
+
 // (sequence, tile) pairs a call can have: every sequence, and the rows behind the last, may end in a partial tile
 int64_t pairs_bound(const PagedAttnArgs& a, int rows) {
   return static_cast<int64_t>(a.p.T) * a.group / rows + std::min<int64_t>(a.p.B + 1, a.p.T);
@@ -1104,11 +1132,11 @@ void launch(const Plan& p, hipStream_t s) {
       const PagedAttnArgs& a = p.t;
       const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(a.slots) * a.hkv);
       if (a.d <= 64)
-        paged_attn_tile<T, 64, 8><<<grid, 512, 0, s>>>(a);
+        launch_tile<T, 64, 8>(a, grid, s);
       else if (a.d <= 128)
-        paged_attn_tile<T, 128, 8><<<grid, 512, 0, s>>>(a);
+        launch_tile<T, 128, 8>(a, grid, s);
       else
-        paged_attn_tile<T, 256, 4><<<grid, 256, 0, s>>>(a);
+        launch_tile<T, 256, 4>(a, grid, s);
       if (a.target > 0) {
         if (a.d <= 128)
           launch_join<T, 256, kTileKeys>(a, pairs_bound(a, 256), s);

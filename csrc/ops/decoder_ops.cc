@@ -89,6 +89,9 @@ Cache check_cache(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     bool ok = t->stride(3) == 1 && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0;
     for (int64_t i = 0; i < 3; ++i) ok = ok && (t->size(i) <= 1 || t->stride(i) * t->element_size() % 16 == 0);
     TORCH_CHECK(ok, op, ": rows of the cache start at multiples of 16 bytes and are packed, got strides ", t->strides());
+    for (int64_t i : {0, 2})
+      TORCH_CHECK(t->size(i) <= 1 || (t->stride(i) >= 0 && t->stride(i) * t->element_size() <= (int64_t{1} << 31)), op,
+                  ": pages and rows of the cache are at most 2 GiB apart, got strides ", t->strides());
   }
   TORCH_CHECK(table.scalar_type() == at::kInt && table.dim() == 2 && table.device() == q.device() &&
                   (table.size(1) <= 1 || table.stride(1) == 1),
