@@ -41,7 +41,6 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
 constexpr int kRows = 32;   // rows of one item
 constexpr int kKeys = 32;   // keys of one block
 constexpr int kCus = 256;
@@ -147,7 +146,8 @@ __device__ __forceinline__ float row_sum(float x) {
 // the sequences.  target = 0: no split.
 struct Item {
   int b;        // sequence; -1: nothing to do.  B: the rows behind the last sequence
-  int tile, split, splits, slot;
+  int tile, split, splits;
+  int part;     // of the scratch memory, if split
   int chunk;    // key blocks of a split
   int n, t0;    // new tokens, first token row
   int len, keys;  // length; keys that the table can hold of them
@@ -198,9 +198,9 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t* t
 }
 
 // PAIRS false: `index` counts items; PAIRS true: (sequence, tile) pairs, and
-// the item's slot is that of the pair's first split
+// the item is the pair's first split
 template <int ROWS, int KEYS, bool PAIRS>
-__device__ Item find_item(const PagedAttnArgs& a, int index, int64_t* sh /* [kWaves] */, int* found /* [kFound] */) {
+__device__ Item find_item(const PagedAttnArgs& a, int index, int64_t* sh /* [waves] */, int* found /* [kFound] */) {
   Item it;
   const int tid = threadIdx.x, nt = blockDim.x, B1 = a.p.B + 1;
   int chunk = 1 << 28;
@@ -216,7 +216,8 @@ __device__ Item find_item(const PagedAttnArgs& a, int index, int64_t* sh /* [kWa
     chunk = static_cast<int>(min(max(c, static_cast<int64_t>(a.min_chunk)), static_cast<int64_t>(1 << 28)));
   }
   if (tid == 0) found[0] = -1;
-  int64_t carry = 0;  // pairs << 32 | items
+  // pairs << 32 | items beyond one a pair << 16 | items of split pairs: the last two are below 2 target
+  int64_t carry = 0;
   for (int b0 = 0; b0 < B1; b0 += nt) {
     const int b = b0 + tid;
     int64_t mine = 0;
@@ -226,26 +227,28 @@ __device__ Item find_item(const PagedAttnArgs& a, int index, int64_t* sh /* [kWa
       if (b0 > 0) s = seq_of<ROWS, KEYS>(a, b);
       tiles = s.tiles;
       splits = max((s.blocks + chunk - 1) / chunk, 1);
-      mine = (static_cast<int64_t>(tiles) << 32) + static_cast<int64_t>(tiles) * splits;
+      mine = (static_cast<int64_t>(tiles) << 32) +
+             (splits > 1 ? static_cast<int64_t>(tiles) * (((splits - 1) << 16) + splits) : 0);
     }
     int64_t total;
     const int64_t first = carry + block_scan(mine, sh, &total);
-    const int first_item = static_cast<int>(first & 0xffffffff), first_pair = static_cast<int>(first >> 32);
+    const int first_pair = static_cast<int>(first >> 32), first_part = static_cast<int>(first & 0xffff);
+    const int first_item = first_pair + static_cast<int>(first >> 16 & 0xffff);
     const int rel = index - (PAIRS ? first_pair : first_item);
     if (rel >= 0 && rel < (PAIRS ? tiles : tiles * splits)) {
-      const int tile = PAIRS ? rel : rel / splits;
+      const int tile = PAIRS ? rel : rel / splits, split = PAIRS ? 0 : rel % splits;
       found[0] = b;
       found[1] = tiles - 1 - tile;  // the tiles with the most keys first: the short ones fill the tail
-      found[2] = PAIRS ? 0 : rel % splits;
+      found[2] = split;
       found[3] = splits;
-      found[4] = first_item + tile * splits + (PAIRS ? 0 : rel % splits);
+      found[4] = first_part + tile * splits + split;
       found[5] = s.n;
       found[6] = s.t0;
       found[7] = s.len;
       found[8] = s.keys;
     }
     carry += total;
-    if (index < (PAIRS ? carry >> 32 : carry & 0xffffffff)) break;  // (the same in every thread)
+    if (index < (PAIRS ? carry >> 32 : (carry >> 32) + (carry >> 16 & 0xffff))) break;  // (the same in every thread)
   }
   __syncthreads();
   it.b = __builtin_amdgcn_readfirstlane(found[0]);
@@ -253,9 +256,9 @@ __device__ Item find_item(const PagedAttnArgs& a, int index, int64_t* sh /* [kWa
   it.tile = __builtin_amdgcn_readfirstlane(found[1]);
   it.split = __builtin_amdgcn_readfirstlane(found[2]);
   it.splits = __builtin_amdgcn_readfirstlane(found[3]);
-  it.slot = __builtin_amdgcn_readfirstlane(found[4]);
-  if (PAIRS && (it.slot < 0 || it.slot > a.slots - it.splits)) {  // (offsets that do not ascend: more items than slots)
-    it.b = -1;
+  it.part = __builtin_amdgcn_readfirstlane(found[4]);
+  if (it.splits > 1 && (it.part < 0 || it.part > 2 * a.target - (PAIRS ? it.splits : 1))) {
+    it.b = -1;  // (offsets that do not ascend: more items than planned for)
     return it;
   }
   it.chunk = __builtin_amdgcn_readfirstlane(chunk);
@@ -295,17 +298,17 @@ __device__ __forceinline__ bool is_there(const PagedAttnArgs& a, const KeyRow& r
   return static_cast<uint32_t>(r.id) < static_cast<uint32_t>(a.p.pages);
 }
 
-// workspace of a split call: per (item slot, kv head) kRows x (d floats) and kRows x (max, sum)
+// scratch memory of a split call: for an item of a split pair and a kv head, rows x (max, sum, d columns)
 __host__ __device__ __forceinline__ size_t part_floats(int rows, int d) { return static_cast<size_t>(rows) * (d + 2); }
 
 // ------------------------------------------------------------ stream kernel ----
-// One workgroup per item of 32 rows; its four waves take key blocks in turn,
+// One workgroup per item of 32 rows; its waves take key blocks in turn,
 // each on its own (no barrier in the loop) and straight from global memory into
 // the matrix instructions' registers: a lane loads 16 bytes of a key for S^T;
 // for O^T the lanes of a half load a whole row of V (DP / 32 neighbouring
 // columns each, so column = (DP / 32) * row of the tile + tile) and eight rows'
-// halves are interleaved with byte permutes.  Four partial (max, sum, O) are
-// joined through LDS at the end.
+// halves are interleaved with byte permutes.  The waves' partial (max, sum,
+// O) are joined through LDS at the end.
 template <typename T>
 struct Elem { using type = uint16_t; static constexpr bool wide = false; };
 template <>
@@ -313,8 +316,8 @@ struct Elem<F32> { using type = float; static constexpr bool wide = true; };
 
 // QUAD: pages hold whole groups of four keys, so four neighbouring rows of V
 // are addressed from the first one's offset.
-template <typename T, int DP, bool QUAD>
-__global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) void paged_attn_stream(PagedAttnArgs a) {
+template <typename T, int DP, bool QUAD, int kWaves>
+__device__ __forceinline__ void stream_item(const PagedAttnArgs& a, unsigned index) {
   using E = typename Elem<T>::type;
   constexpr bool WIDE = Elem<T>::wide;
   constexpr int NB = DP / 32;            // 32-column tiles of O^T
@@ -323,12 +326,12 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
   __shared__ int64_t sh_scan[kWaves];
   __shared__ int sh_found[kFound];
   __shared__ float sh_ml[kWaves][2][kRows];
-  __shared__ float sh_o[2][NB * 16][64];
+  __shared__ float sh_o[kWaves / 2][NB * 16][64];
   constexpr bool QLDS = DP * sizeof(E) > 256;
   __shared__ u32x4 sh_q[QLDS ? KC : 1][64];
 
-  const int head = static_cast<int>(blockIdx.x % a.hkv);
-  const int slot = static_cast<int>(blockIdx.x / a.hkv);
+  const int head = static_cast<int>(index % a.hkv);
+  const int slot = static_cast<int>(index / a.hkv);
   const Item it = find_item<kRows, kKeys, false>(a, slot, sh_scan, sh_found);
   if (it.b < 0) return;
 
@@ -553,7 +556,7 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
   }
   sum = row_sum(sum);
 
-  // join the waves: a common maximum, then O in two rounds (2, 3 -> 0, 1; 1 -> 0)
+  // join the waves: a common maximum, then O in rounds, the upper half of the waves to the lower
   if (half == 0) {
     sh_ml[wave][0][col] = mx;
     sh_ml[wave][1][col] = sum;
@@ -571,7 +574,7 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[m][i] *= f;
 #pragma unroll
-  for (int r = 2; r >= 1; r >>= 1) {
+  for (int r = kWaves / 2; r >= 1; r >>= 1) {
     if (wave >= r && wave < 2 * r) {
 #pragma unroll
       for (int m = 0; m < NB; ++m)
@@ -590,7 +593,7 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
   if (wave != 0 || !live) return;
 
   if (it.splits > 1) {
-    float* ws = static_cast<float*>(a.ws) + (static_cast<size_t>(slot) * a.hkv + head) * part_floats(kRows, a.d);
+    float* ws = static_cast<float*>(a.ws) + (static_cast<size_t>(it.part) * a.hkv + head) * part_floats(kRows, a.d);
     if (half == 0) {
       ws[col] = M;
       ws[kRows + col] = L;
@@ -624,6 +627,11 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
   }
 }
 
+template <typename T, int DP, bool QUAD>
+__global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) void paged_attn_stream(PagedAttnArgs a) {
+  stream_item<T, DP, QUAD, kThreads / 64>(a, blockIdx.x);
+}
+
 // -------------------------------------------------------------- tile kernel ----
 // Many rows of one sequence: a workgroup of WAVES waves takes 32 rows each and
 // all walk over the same key blocks of 64, staged through LDS in two buffers: a
@@ -646,7 +654,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 #define NNSX_GLOBAL __attribute__((address_space(1)))
 
 template <typename T, int DP, int WAVES, bool ONE_PAGE>
-__global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile(PagedAttnArgs a) {
+__device__ __forceinline__ void tile_item(const PagedAttnArgs& a, unsigned index) {
   using E = uint16_t;
   constexpr int ROWS = WAVES * 32, NB = DP / 32, KC = DP / 16, P = DP / 8;
   constexpr int PASS = WAVES * 64 / P;       // rows of a block that the workgroup loads at once,
@@ -660,8 +668,8 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
   // of a row are reached by exclusive or.
   constexpr int ROW = DP * 2, TILE = kTileKeys * ROW;
   __shared__ __attribute__((aligned(1024))) char sh_k0[TILE], sh_k1[TILE], sh_v0[TILE], sh_v1[TILE];
-  const int head = static_cast<int>(blockIdx.x % a.hkv);
-  const int slot = static_cast<int>(blockIdx.x / a.hkv);
+  const int head = static_cast<int>(index % a.hkv);
+  const int slot = static_cast<int>(index / a.hkv);
   const Item it = find_item<ROWS, kTileKeys, false>(a, slot, sh_scan, sh_found);
   if (it.b < 0) return;
 
@@ -940,7 +948,7 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
   if (!live) return;
 
   if (it.splits > 1) {
-    float* ws = static_cast<float*>(a.ws) + (static_cast<size_t>(slot) * a.hkv + head) * part_floats(ROWS, a.d);
+    float* ws = static_cast<float*>(a.ws) + (static_cast<size_t>(it.part) * a.hkv + head) * part_floats(ROWS, a.d);
     const int r = wave * 32 + col;
     if (half == 0) {
       ws[r] = mx;
@@ -969,37 +977,52 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
     }
 }
 
+template <typename T, int DP, int WAVES, bool ONE_PAGE>
+__global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile(PagedAttnArgs a) {
+  tile_item<T, DP, WAVES, ONE_PAGE>(a, blockIdx.x);
+}
+
+// A batch of long and short pieces: the tile form's items first, the stream form's after them, one launch.
+template <typename T, int DP, bool ONE_PAGE>
+__global__ __launch_bounds__(512, 2) void paged_attn_both(PagedAttnArgs t, PagedAttnArgs s, unsigned tiles) {
+  if (blockIdx.x < tiles)
+    tile_item<T, DP, 8, ONE_PAGE>(t, blockIdx.x);
+  else
+    stream_item<T, DP, ONE_PAGE, 8>(s, blockIdx.x - tiles);
+}
+
 // ------------------------------------------------------------------- join ----
 // Joins the splits of one (sequence, tile, kv head):
 //   M = max_s m_s,  o = sum_s e^(m_s - M) o_s / sum_s e^(m_s - M) l_s.
 // LG lanes hold a row's columns, four each; the workgroup's 256 / LG such
 // groups divide the live rows and, where there are few, a row's splits, whose
-// parts are added through LDS in a fixed order.  blockIdx.y takes every
-// gridDim.y-th row: few pairs are spread over more workgroups.
+// parts are added through LDS in a fixed order.  A pair's rows are dealt out to
+// a.apart workgroups: few pairs are spread over more of the card.
 constexpr int kJoinThreads = 256;
 
 template <typename T, int ROWS, int KEYS, int LG>
-__global__ __launch_bounds__(kJoinThreads) void paged_attn_join(PagedAttnArgs a) {
+__device__ __forceinline__ void join_pair(const PagedAttnArgs& a, unsigned index) {
   using E = typename Elem<T>::type;
   constexpr int NG = kJoinThreads / LG;
   __shared__ int64_t sh_scan[kJoinThreads / 64];
   __shared__ int sh_found[kFound];
   __shared__ f32x4 sh_o[NG][LG];
   __shared__ float sh_l[NG];
-  const int head = static_cast<int>(blockIdx.x % a.hkv);
-  const Item it = find_item<ROWS, KEYS, true>(a, static_cast<int>(blockIdx.x / a.hkv), sh_scan, sh_found);
+  const int apart = a.apart, mine = static_cast<int>(index % apart);
+  const int head = static_cast<int>(index / apart % a.hkv);
+  const Item it = find_item<ROWS, KEYS, true>(a, static_cast<int>(index / apart / a.hkv), sh_scan, sh_found);
   if (it.b < 0 || it.splits == 1) return;
   const int lg = threadIdx.x % LG, grp = threadIdx.x / LG;
-  const int all = min(it.n * a.group - it.tile * ROWS, ROWS), apart = static_cast<int>(gridDim.y);
-  const int live = (all - static_cast<int>(blockIdx.y) + apart - 1) / apart;  // rows of this workgroup
+  const int all = min(it.n * a.group - it.tile * ROWS, ROWS);
+  const int live = (all - mine + apart - 1) / apart;  // rows of this workgroup
   if (live <= 0) return;
   int per_row = NG;  // groups of a row: a power of two
   while (per_row > 1 && per_row * live > NG) per_row >>= 1;
   const int rows_at_once = NG / per_row, part = grp % per_row;
   const size_t step = static_cast<size_t>(a.hkv) * part_floats(ROWS, a.d);
-  const float* ws = static_cast<const float*>(a.ws) + (static_cast<size_t>(it.slot) * a.hkv + head) * part_floats(ROWS, a.d);
+  const float* ws = static_cast<const float*>(a.ws) + (static_cast<size_t>(it.part) * a.hkv + head) * part_floats(ROWS, a.d);
   for (int r0 = 0; r0 < live; r0 += rows_at_once) {
-    const int i0 = r0 + grp / per_row, r = i0 * apart + static_cast<int>(blockIdx.y);
+    const int i0 = r0 + grp / per_row, r = i0 * apart + mine;
     f32x4 acc = (f32x4)(0.f);
     float L = 0.f;
     if (i0 < live) {
@@ -1044,27 +1067,32 @@ __global__ __launch_bounds__(kJoinThreads) void paged_attn_join(PagedAttnArgs a)
   }
 }
 
-template <typename T, int ROWS, int KEYS>
-void launch_join(const PagedAttnArgs& a, int64_t pairs, hipStream_t s) {
-  const int64_t wgs = pairs * a.hkv;
-  const dim3 grid(static_cast<unsigned>(wgs), static_cast<unsigned>(std::clamp<int64_t>(4 * kCus / wgs, 1, ROWS)));
-  if (a.d <= 64)
-    paged_attn_join<T, ROWS, KEYS, 16><<<grid, kJoinThreads, 0, s>>>(a);
-  else if (a.d <= 128)
-    paged_attn_join<T, ROWS, KEYS, 32><<<grid, kJoinThreads, 0, s>>>(a);
-  else
-    paged_attn_join<T, ROWS, KEYS, 64><<<grid, kJoinThreads, 0, s>>>(a);
+// `tiles` workgroups for the tile form's pairs, then the stream form's
+template <typename T, int TILE_ROWS, int LG>
+__global__ __launch_bounds__(kJoinThreads) void paged_attn_join(PagedAttnArgs t, PagedAttnArgs s, unsigned tiles) {
+  if constexpr (TILE_ROWS > 0) {
+    if (blockIdx.x < tiles) return join_pair<T, TILE_ROWS, kTileKeys, LG>(t, blockIdx.x);
+  }
+  join_pair<T, kRows, kKeys, LG>(s, blockIdx.x - tiles);
 }
 
-template <typename T, bool QUAD>
+template <typename T, int DP>
+void launch_stream(const PagedAttnArgs& a, unsigned grid, hipStream_t s) {
+  if (a.p.page % 4 == 0)
+    paged_attn_stream<T, DP, true><<<grid, kThreads, 0, s>>>(a);
+  else
+    paged_attn_stream<T, DP, false><<<grid, kThreads, 0, s>>>(a);
+}
+
+template <typename T>
 void launch_stream(const PagedAttnArgs& a, hipStream_t s) {
   const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(a.slots) * a.hkv);
   if (a.d <= 64)
-    paged_attn_stream<T, 64, QUAD><<<grid, kThreads, 0, s>>>(a);
+    launch_stream<T, 64>(a, grid, s);
   else if (a.d <= 128)
-    paged_attn_stream<T, 128, QUAD><<<grid, kThreads, 0, s>>>(a);
+    launch_stream<T, 128>(a, grid, s);
   else
-    paged_attn_stream<T, 256, QUAD><<<grid, kThreads, 0, s>>>(a);
+    launch_stream<T, 256>(a, grid, s);
 }
 
 template <typename T, int DP, int WAVES>
@@ -1082,26 +1110,26 @@ int64_t pairs_bound(const PagedAttnArgs& a, int rows) {
 
 int tile_rows(const PagedAttnArgs& a) { return a.d <= 128 ? 256 : 128; }
 
-// One launch of either kernel: which sequences it takes (by their rows), how
-// its keys are split, its scratch memory.  Enough whole tiles to fill the card:
-// no split.  Otherwise about `per_cu` workgroups a compute unit, of at least `min_chunk` key blocks.
-PagedAttnArgs part_of(const PagedAttnArgs& a0, int rows, int rows_lo, int rows_hi, int per_cu, int min_chunk) {
+// Either form's part of a call: which sequences it takes (by their rows), and
+// how its keys are split: for about `target` items a kv head (0: no split), of at least `min_chunk` key blocks.
+PagedAttnArgs part_of(const PagedAttnArgs& a0, int rows, int rows_lo, int rows_hi, int target, int min_chunk) {
   PagedAttnArgs a = a0;
   a.rows_lo = rows_lo;
   a.rows_hi = rows_hi;
-  const int64_t full = (static_cast<int64_t>(a.p.T) * a.group + rows - 1) / rows * a.hkv;
-  a.target = full >= 2 * per_cu * kCus ? 0 : (per_cu * kCus + a.hkv - 1) / a.hkv;
+  a.target = (target + a.hkv - 1) / a.hkv;
   a.min_chunk = min_chunk;
-  a.slots = static_cast<int>(pairs_bound(a, rows) + a.target);
+  a.pairs = static_cast<int>(pairs_bound(a, rows));
+  a.slots = a.pairs + a.target;
+  a.apart = static_cast<int>(std::clamp<int64_t>(4 * kCus / (static_cast<int64_t>(a.pairs) * a.hkv), 1, rows));
   return a;
 }
 
 size_t part_bytes(const PagedAttnArgs& a, int rows) {
-  return a.target == 0 ? 0 : static_cast<size_t>(a.slots) * a.hkv * part_floats(rows, a.d) * sizeof(float);
+  return static_cast<size_t>(2 * a.target) * a.hkv * part_floats(rows, a.d) * sizeof(float);
 }
 
 constexpr int kAllRows = 0x7fffffff;
-// Rows of a sequence up to which the stream kernel takes it
+// Rows of a sequence up to which the stream form takes it
 constexpr int kStreamRows = 64;
 
 struct Plan {
@@ -1112,47 +1140,70 @@ struct Plan {
 Plan plan_of(PagedAttnArgs a) {
   a.group = a.hq / a.hkv;
   Plan p;
-  // One token a sequence on average: the stream kernel takes every sequence.
-  // A single sequence is one kernel's.  Else both run, each on its own sequences.
+  // One token a sequence on average: the stream form takes every sequence.
+  // A single sequence is one form's.  Else both run, each on its own sequences.
   if (a.type == AttnType::kF32 || a.p.T <= a.p.B)
     p.tile = false;
   else
     p.tile = a.p.B > 1 || static_cast<int64_t>(a.p.T) * a.group > kStreamRows;
   p.stream = !p.tile || a.p.B > 1;
-  p.s = part_of(a, kRows, 0, p.tile ? kStreamRows : kAllRows, 4, 4);
-  p.t = part_of(a, tile_rows(a), p.stream ? kStreamRows : 0, kAllRows, 1, 4);
+  // The stream form always splits: a sequence much longer than the others is spread over the card.
+  p.s = part_of(a, kRows, 0, p.tile ? kStreamRows : kAllRows, (p.tile ? 2 : 4) * kCus, p.tile ? 8 : 4);
+  if (p.tile) {  // (two tiles a sequence at most, and the rows behind the last)
+    p.s.pairs = static_cast<int>(std::min<int64_t>(p.s.pairs, 2 * (static_cast<int64_t>(a.p.B) + 1)));
+    p.s.slots = p.s.pairs + p.s.target;
+  }
+  // The tile form where whole tiles do not fill the card.
+  const int64_t tiles = (static_cast<int64_t>(a.p.T) * a.group + tile_rows(a) - 1) / tile_rows(a) * a.hkv;
+  p.t = part_of(a, tile_rows(a), p.stream ? kStreamRows : 0, kAllRows, tiles >= 2 * kCus ? 0 : kCus, 4);
   p.t.ws = static_cast<char*>(a.ws) + (p.stream ? part_bytes(p.s, kRows) : 0);
   return p;
+}
+
+unsigned grid_of(const PagedAttnArgs& a) { return static_cast<unsigned>(static_cast<int64_t>(a.slots) * a.hkv); }
+
+template <typename T, int TILE_ROWS>
+void launch_join(const Plan& p, hipStream_t s) {
+  const auto wgs = [](bool runs, const PagedAttnArgs& a) {
+    return runs && a.target > 0 ? static_cast<unsigned>(static_cast<int64_t>(a.pairs) * a.hkv * a.apart) : 0u;
+  };
+  const unsigned tiles = wgs(p.tile, p.t), grid = tiles + wgs(p.stream, p.s);
+  if (grid == 0) return;
+  if (p.s.d <= 64)
+    paged_attn_join<T, TILE_ROWS, 16><<<grid, kJoinThreads, 0, s>>>(p.t, p.s, tiles);
+  else if (p.s.d <= 128)
+    paged_attn_join<T, TILE_ROWS, 32><<<grid, kJoinThreads, 0, s>>>(p.t, p.s, tiles);
+  else
+    paged_attn_join<T, TILE_ROWS, 64><<<grid, kJoinThreads, 0, s>>>(p.t, p.s, tiles);
+}
+
+template <typename T, int DP>
+void launch_both(const Plan& p, hipStream_t s) {
+  const unsigned tiles = grid_of(p.t), grid = tiles + grid_of(p.s);
+  if (p.t.p.page % (512 / DP) == 0)
+    paged_attn_both<T, DP, true><<<grid, 512, 0, s>>>(p.t, p.s, tiles);
+  else
+    paged_attn_both<T, DP, false><<<grid, 512, 0, s>>>(p.t, p.s, tiles);
 }
 
 template <typename T>
 void launch(const Plan& p, hipStream_t s) {
   if constexpr (!Elem<T>::wide) {
     if (p.tile) {
-      const PagedAttnArgs& a = p.t;
-      const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(a.slots) * a.hkv);
-      if (a.d <= 64)
-        launch_tile<T, 64, 8>(a, grid, s);
-      else if (a.d <= 128)
-        launch_tile<T, 128, 8>(a, grid, s);
-      else
-        launch_tile<T, 256, 4>(a, grid, s);
-      if (a.target > 0) {
-        if (a.d <= 128)
-          launch_join<T, 256, kTileKeys>(a, pairs_bound(a, 256), s);
-        else
-          launch_join<T, 128, kTileKeys>(a, pairs_bound(a, 128), s);
+      if (p.s.d > 128) {  // (the two forms' LDS does not fit one workgroup)
+        launch_tile<T, 256, 4>(p.t, grid_of(p.t), s);
+        if (p.stream) launch_stream<T>(p.s, s);
+        return launch_join<T, 128>(p, s);
       }
+      if (p.s.d <= 64)
+        p.stream ? launch_both<T, 64>(p, s) : launch_tile<T, 64, 8>(p.t, grid_of(p.t), s);
+      else
+        p.stream ? launch_both<T, 128>(p, s) : launch_tile<T, 128, 8>(p.t, grid_of(p.t), s);
+      return launch_join<T, 256>(p, s);
     }
   }
-  if (p.stream) {
-    const PagedAttnArgs& a = p.s;
-    if (a.p.page % 4 == 0)
-      launch_stream<T, true>(a, s);
-    else
-      launch_stream<T, false>(a, s);
-    if (a.target > 0) launch_join<T, kRows, kKeys>(a, pairs_bound(a, kRows), s);
-  }
+  launch_stream<T>(p.s, s);
+  launch_join<T, 0>(p, s);
 }
 
 }  // namespace
