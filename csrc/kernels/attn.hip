@@ -44,7 +44,6 @@ constexpr int kThreads = 256;
 constexpr int kRows = 32;   // rows of one item
 constexpr int kKeys = 32;   // keys of one block
 constexpr int kCus = 256;
-constexpr int kFound = 9;   // ints of LDS that find_item passes an item through
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_huge_valf();
 
@@ -139,11 +138,11 @@ __device__ __forceinline__ float row_sum(float x) {
 
 // ------------------------------------------------------------------- plan ----
 // Work is cut into items: (sequence, tile of rows, split of its key blocks).
-// Lengths live on the device, so every workgroup derives its own item from
-// them: the key blocks of all (sequence, tile) pairs are summed, a split is
-// chosen so long that about `target` items result (more only because every
-// pair has at least one), and the item's pair is found by a running sum over
-// the sequences.  target = 0: no split.
+// Lengths live on the device, so every wave derives its own item from them: the
+// key blocks of all (sequence, tile) pairs are summed, a split is chosen so long
+// that about `target` items result (more only because every pair has at least
+// one), and the item's pair is found by a running sum over the sequences.
+// target = 0: no split.
 struct Item {
   int b;        // sequence; -1: nothing to do.  B: the rows behind the last sequence
   int tile, split, splits;
@@ -160,112 +159,115 @@ struct Seq {
 template <int ROWS, int KEYS>
 __device__ __forceinline__ Seq seq_of(const PagedAttnArgs& a, int b) {
   Seq s;
-  const int T = a.p.T;
-  auto at = [&](int i) { return i == 0 ? 0 : min(max(a.p.cu[i], 0), T); };
-  s.t0 = at(b);
-  const int t1 = b < a.p.B ? at(b + 1) : T;
+  const int T = a.p.T, B = a.p.B;
+  // (three loads at once; the last entry stands for the rows behind the last sequence)
+  const int c0 = a.p.cu[b], c1 = a.p.cu[min(b + 1, B)], len = B > 0 ? a.p.len[min(b, B - 1)] : 0;
+  s.t0 = b == 0 ? 0 : min(max(c0, 0), T);
+  const int t1 = b < B ? min(max(c1, 0), T) : T;
   s.n = max(t1 - s.t0, 0);
-  s.len = b < a.p.B ? max(a.p.len[b], 0) : 0;
-  s.keys = static_cast<int>(min(static_cast<int64_t>(s.len), static_cast<int64_t>(a.p.width) * a.p.page));
-  const int64_t rows = static_cast<int64_t>(s.n) * a.group;
-  if (rows <= a.rows_lo || rows > a.rows_hi) s.n = 0;  // (another launch's)
-  s.tiles = s.n > 0 ? static_cast<int>((rows + ROWS - 1) / ROWS) : 0;
-  const int64_t first = static_cast<int64_t>(s.len) - s.n - a.window + 1;  // first key the first token sees
-  const int lo = a.window > 0 ? static_cast<int>(min(max(first, static_cast<int64_t>(0)), static_cast<int64_t>(s.keys))) : 0;
-  s.blocks = s.n > 0 ? (s.keys + KEYS - 1) / KEYS - lo / KEYS : 0;
+  s.len = b < B ? max(len, 0) : 0;
+  s.keys = min(s.len, a.p.width * a.p.page);
+  const int rows = s.n * a.group;  // (T * hq < 2^31)
+  if (rows <= a.rows_lo || rows > a.rows_hi) s.n = 0;  // (the other form's)
+  s.tiles = s.n > 0 ? static_cast<int>((static_cast<uint32_t>(rows) + ROWS - 1) / ROWS) : 0;
+  const int lo = a.window > 0 ? min(max(s.len - s.n - a.window + 1, 0), s.keys) : 0;
+  s.blocks = s.n > 0 ? static_cast<int>(static_cast<uint32_t>(s.keys + KEYS - 1) / KEYS - static_cast<uint32_t>(lo) / KEYS) : 0;
   return s;
 }
 
-// value and running sum over the workgroup (wave shuffles, then the waves' sums)
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t* total) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int64_t x = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
-  __syncthreads();
-  if (lane == 63) sh[w] = x;
-  __syncthreads();
-  int64_t base = 0, sum = 0;
-  for (int i = 0; i < static_cast<int>(blockDim.x >> 6); ++i) {
-    if (i < w) base += sh[i];
-    sum += sh[i];
-  }
-  *total = sum;
-  return base + x - v;  // exclusive
+// sum of the lanes up to this one
+template <typename V>
+__device__ __forceinline__ V wave_scan(V x) {
+  auto shifted = [&](auto ctrl, auto rows) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value,
+                                                             decltype(rows)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  x += shifted(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});  // row_shr 1, 2, 4, 8
+  x += shifted(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  x += shifted(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  x += shifted(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  x += shifted(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // row_bcast 15, 31
+  x += shifted(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
+  return x;
+}
+template <typename V>
+__device__ __forceinline__ V last_lane(V x) {
+  return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+
+// key blocks of a split: the items of all pairs stay within `target` more than the pairs
+__device__ __forceinline__ int chunk_of(const PagedAttnArgs& a, float blocks) {
+  if (a.target == 0) return 1 << 28;
+  // (a float sum of few terms is off by less than the 1e-4 that is added)
+  const float c = blocks * 1.0001f / static_cast<float>(a.target);
+  return max(static_cast<int>(fminf(c, 2e8f)) + 1, a.min_chunk);
+}
+
+// pairs, items beyond one a pair << 16 | items of split pairs (both below 2 target)
+struct Count {
+  int pairs;
+  uint32_t split;
+};
+__device__ __forceinline__ Count count_of(const Seq& s, int splits) {
+  return {s.tiles, splits > 1 ? static_cast<uint32_t>(s.tiles) * (static_cast<uint32_t>(splits - 1) << 16 | splits) : 0u};
+}
+__device__ __forceinline__ int splits_of(const Seq& s, int chunk) {
+  return s.blocks > chunk ? static_cast<int>(static_cast<uint32_t>(s.blocks + chunk - 1) / static_cast<uint32_t>(chunk)) : 1;
 }
 
 // PAIRS false: `index` counts items; PAIRS true: (sequence, tile) pairs, and
-// the item is the pair's first split
+// the item is the pair's first split.  Each wave finds it by itself among 64
+// sequences at a time; more are summed up first, 64 at a time, by every wave.
 template <int ROWS, int KEYS, bool PAIRS>
-__device__ Item find_item(const PagedAttnArgs& a, int index, int64_t* sh /* [waves] */, int* found /* [kFound] */) {
+__device__ Item find_item(const PagedAttnArgs& a, int index) {
   Item it;
-  const int tid = threadIdx.x, nt = blockDim.x, B1 = a.p.B + 1;
-  int chunk = 1 << 28;
-  const Seq mine0 = tid < B1 ? seq_of<ROWS, KEYS>(a, tid) : Seq{};
-  if (a.target > 0) {
-    int64_t w = static_cast<int64_t>(mine0.tiles) * mine0.blocks, total;
-    for (int b = tid + nt; b < B1; b += nt) {
-      const Seq s = seq_of<ROWS, KEYS>(a, b);
-      w += static_cast<int64_t>(s.tiles) * s.blocks;
+  it.b = -1;
+  const int lane = threadIdx.x & 63, B1 = a.p.B + 1;
+  Seq s{};
+  if (lane < B1) s = seq_of<ROWS, KEYS>(a, lane);
+  float work = static_cast<float>(s.tiles) * static_cast<float>(s.blocks);
+  if (a.target > 0)
+    for (int b = lane + 64; b < B1; b += 64) {
+      const Seq x = seq_of<ROWS, KEYS>(a, b);
+      work += static_cast<float>(x.tiles) * static_cast<float>(x.blocks);
     }
-    block_scan(w, sh, &total);
-    const int64_t c = (total + a.target - 1) / a.target;
-    chunk = static_cast<int>(min(max(c, static_cast<int64_t>(a.min_chunk)), static_cast<int64_t>(1 << 28)));
-  }
-  if (tid == 0) found[0] = -1;
-  // pairs << 32 | items beyond one a pair << 16 | items of split pairs: the last two are below 2 target
-  int64_t carry = 0;
-  for (int b0 = 0; b0 < B1; b0 += nt) {
-    const int b = b0 + tid;
-    int64_t mine = 0;
-    int tiles = 0, splits = 1;
-    Seq s = mine0;
-    if (b < B1) {
-      if (b0 > 0) s = seq_of<ROWS, KEYS>(a, b);
-      tiles = s.tiles;
-      splits = max((s.blocks + chunk - 1) / chunk, 1);
-      mine = (static_cast<int64_t>(tiles) << 32) +
-             (splits > 1 ? static_cast<int64_t>(tiles) * (((splits - 1) << 16) + splits) : 0);
+  const int chunk = chunk_of(a, last_lane(wave_scan(work)));
+  Count before{0, 0};
+  for (int b0 = 0; b0 < B1; b0 += 64) {
+    if (b0 > 0) {
+      s = Seq{};
+      if (b0 + lane < B1) s = seq_of<ROWS, KEYS>(a, b0 + lane);
     }
-    int64_t total;
-    const int64_t first = carry + block_scan(mine, sh, &total);
-    const int first_pair = static_cast<int>(first >> 32), first_part = static_cast<int>(first & 0xffff);
-    const int first_item = first_pair + static_cast<int>(first >> 16 & 0xffff);
-    const int rel = index - (PAIRS ? first_pair : first_item);
-    if (rel >= 0 && rel < (PAIRS ? tiles : tiles * splits)) {
-      const int tile = PAIRS ? rel : rel / splits, split = PAIRS ? 0 : rel % splits;
-      found[0] = b;
-      found[1] = tiles - 1 - tile;  // the tiles with the most keys first: the short ones fill the tail
-      found[2] = split;
-      found[3] = splits;
-      found[4] = first_part + tile * splits + split;
-      found[5] = s.n;
-      found[6] = s.t0;
-      found[7] = s.len;
-      found[8] = s.keys;
+    const int splits = splits_of(s, chunk);
+    const Count mine = count_of(s, splits);
+    const int pairs = wave_scan(mine.pairs);
+    const uint32_t split = a.target > 0 ? static_cast<uint32_t>(wave_scan(static_cast<int>(mine.split))) : 0u;
+    const int first_pair = before.pairs + pairs - mine.pairs;
+    const uint32_t first_split = before.split + split - mine.split;
+    const int first = PAIRS ? first_pair : first_pair + static_cast<int>(first_split >> 16);
+    const uint64_t here = __ballot(index >= first && index - first < s.tiles * (PAIRS ? 1 : splits));
+    if (here != 0) {
+      const int l = __builtin_ctzll(here);
+      auto get = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+      const int rel = index - get(first);
+      it.splits = get(splits);
+      const int tile = PAIRS ? rel : rel / it.splits;
+      it.split = PAIRS ? 0 : rel - tile * it.splits;
+      it.tile = get(s.tiles) - 1 - tile;  // the tiles with the most keys first: the short ones fill the tail
+      it.part = (get(static_cast<int>(first_split)) & 0xffff) + tile * it.splits + it.split;
+      it.chunk = chunk;
+      it.n = get(s.n);
+      it.t0 = get(s.t0);
+      it.len = get(s.len);
+      it.keys = get(s.keys);
+      // (offsets that do not ascend may make more items than planned for: those are left out)
+      if (it.splits == 1 || (it.part >= 0 && it.part <= 2 * a.target - (PAIRS ? it.splits : 1))) it.b = b0 + l;
+      return it;
     }
-    carry += total;
-    if (index < (PAIRS ? carry >> 32 : (carry >> 32) + (carry >> 16 & 0xffff))) break;  // (the same in every thread)
+    before.pairs += last_lane(pairs);
+    before.split += static_cast<uint32_t>(last_lane(static_cast<int>(split)));
   }
-  __syncthreads();
-  it.b = __builtin_amdgcn_readfirstlane(found[0]);
-  if (it.b < 0) return it;
-  it.tile = __builtin_amdgcn_readfirstlane(found[1]);
-  it.split = __builtin_amdgcn_readfirstlane(found[2]);
-  it.splits = __builtin_amdgcn_readfirstlane(found[3]);
-  it.part = __builtin_amdgcn_readfirstlane(found[4]);
-  if (it.splits > 1 && (it.part < 0 || it.part > 2 * a.target - (PAIRS ? it.splits : 1))) {
-    it.b = -1;  // (offsets that do not ascend: more items than planned for)
-    return it;
-  }
-  it.chunk = __builtin_amdgcn_readfirstlane(chunk);
-  it.n = __builtin_amdgcn_readfirstlane(found[5]);
-  it.t0 = __builtin_amdgcn_readfirstlane(found[6]);
-  it.len = __builtin_amdgcn_readfirstlane(found[7]);
-  it.keys = __builtin_amdgcn_readfirstlane(found[8]);
   return it;
 }
 
@@ -323,8 +325,6 @@ __device__ __forceinline__ void stream_item(const PagedAttnArgs& a, unsigned ind
   constexpr int NB = DP / 32;            // 32-column tiles of O^T
   constexpr int KC = WIDE ? DP / 8 : DP / 16;  // 16-byte pieces of a key per lane
   constexpr int PIECE = WIDE ? 4 : 8;    // elements of a piece
-  __shared__ int64_t sh_scan[kWaves];
-  __shared__ int sh_found[kFound];
   __shared__ float sh_ml[kWaves][2][kRows];
   __shared__ float sh_o[kWaves / 2][NB * 16][64];
   constexpr bool QLDS = DP * sizeof(E) > 256;
@@ -332,7 +332,7 @@ __device__ __forceinline__ void stream_item(const PagedAttnArgs& a, unsigned ind
 
   const int head = static_cast<int>(index % a.hkv);
   const int slot = static_cast<int>(index / a.hkv);
-  const Item it = find_item<kRows, kKeys, false>(a, slot, sh_scan, sh_found);
+  const Item it = find_item<kRows, kKeys, false>(a, slot);
   if (it.b < 0) return;
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -661,8 +661,6 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, unsigned index
   constexpr int RUN = 64 / P;                // a wave's of them (1 KiB)
   constexpr int PASSES = kTileKeys / PASS;
   static_assert(PASS * PASSES == kTileKeys && RUN * P == 64 && PASSES <= 64, "tile");
-  __shared__ int64_t sh_scan[WAVES];
-  __shared__ int sh_found[kFound];
   // K and V of two blocks, an array each: the compiler keeps them apart, so that a read of one
   // does not wait for the loads into another.  Rows are aligned to their size, so that pieces
   // of a row are reached by exclusive or.
@@ -670,7 +668,7 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, unsigned index
   __shared__ __attribute__((aligned(1024))) char sh_k0[TILE], sh_k1[TILE], sh_v0[TILE], sh_v1[TILE];
   const int head = static_cast<int>(index % a.hkv);
   const int slot = static_cast<int>(index / a.hkv);
-  const Item it = find_item<ROWS, kTileKeys, false>(a, slot, sh_scan, sh_found);
+  const Item it = find_item<ROWS, kTileKeys, false>(a, slot);
   if (it.b < 0) return;
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1004,13 +1002,11 @@ template <typename T, int ROWS, int KEYS, int LG>
 __device__ __forceinline__ void join_pair(const PagedAttnArgs& a, unsigned index) {
   using E = typename Elem<T>::type;
   constexpr int NG = kJoinThreads / LG;
-  __shared__ int64_t sh_scan[kJoinThreads / 64];
-  __shared__ int sh_found[kFound];
   __shared__ f32x4 sh_o[NG][LG];
   __shared__ float sh_l[NG];
   const int apart = a.apart, mine = static_cast<int>(index % apart);
   const int head = static_cast<int>(index / apart % a.hkv);
-  const Item it = find_item<ROWS, KEYS, true>(a, static_cast<int>(index / apart / a.hkv), sh_scan, sh_found);
+  const Item it = find_item<ROWS, KEYS, true>(a, static_cast<int>(index / apart / a.hkv));
   if (it.b < 0 || it.splits == 1) return;
   const int lg = threadIdx.x % LG, grp = threadIdx.x / LG;
   const int all = min(it.n * a.group - it.tile * ROWS, ROWS);
@@ -1120,7 +1116,7 @@ PagedAttnArgs part_of(const PagedAttnArgs& a0, int rows, int rows_lo, int rows_h
   a.min_chunk = min_chunk;
   a.pairs = static_cast<int>(pairs_bound(a, rows));
   a.slots = a.pairs + a.target;
-  a.apart = static_cast<int>(std::clamp<int64_t>(4 * kCus / (static_cast<int64_t>(a.pairs) * a.hkv), 1, rows));
+  a.apart = static_cast<int>(std::clamp<int64_t>(rows / kRows * 4 * kCus / (static_cast<int64_t>(a.pairs) * a.hkv), 1, 32));
   return a;
 }
 
@@ -1148,7 +1144,7 @@ Plan plan_of(PagedAttnArgs a) {
     p.tile = a.p.B > 1 || static_cast<int64_t>(a.p.T) * a.group > kStreamRows;
   p.stream = !p.tile || a.p.B > 1;
   // The stream form always splits: a sequence much longer than the others is spread over the card.
-  p.s = part_of(a, kRows, 0, p.tile ? kStreamRows : kAllRows, (p.tile ? 2 : 4) * kCus, p.tile ? 8 : 4);
+  p.s = part_of(a, kRows, 0, p.tile ? kStreamRows : kAllRows, (p.tile ? 2 : 8) * kCus, p.tile ? 8 : 4);
   if (p.tile) {  // (two tiles a sequence at most, and the rows behind the last)
     p.s.pairs = static_cast<int>(std::min<int64_t>(p.s.pairs, 2 * (static_cast<int64_t>(a.p.B) + 1)));
     p.s.slots = p.s.pairs + p.s.target;

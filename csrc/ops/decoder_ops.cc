@@ -100,9 +100,9 @@ Cache check_cache(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
   check_ints(len, q, table.size(0), op, "kv_lens");
   check_ints(cu, q, table.size(0) + 1, op, "cu_seqlens");
   constexpr int64_t kMax = std::numeric_limits<int>::max();
-  TORCH_CHECK(c.pages <= kMax && table.size(1) * c.page <= kMax - 512 && q.size(0) * q.size(1) <= kMax &&
+  TORCH_CHECK(c.pages <= kMax && table.size(1) * c.page <= (1 << 30) && q.size(0) * q.size(1) <= (1 << 30) &&
                   (q.size(0) + table.size(0) + 1) * c.heads * 16 <= kMax,
-              op, ": more tokens, sequences, pages or positions of a sequence than 31 bits count");
+              op, ": more tokens, sequences, pages or positions of a sequence than 30 bits count");
   return c;
 }
 
@@ -179,7 +179,7 @@ at::Tensor paged_attention_cuda(const at::Tensor& q0, const at::Tensor& k, const
   a.d = static_cast<int>(call.c.dim);
   a.scale = static_cast<float>(call.scale);
   a.causal = causal ? 1 : 0;
-  a.window = static_cast<int>(std::min<int64_t>(window, std::numeric_limits<int>::max()));
+  a.window = window < (1 << 30) ? static_cast<int>(window) : 0;  // (no position is farther)
   at::Tensor ws;
   if (const size_t bytes = nnsx::kernels::paged_attn_workspace_bytes(a)) {
     ws = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
