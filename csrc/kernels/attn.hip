@@ -1003,7 +1003,7 @@ __device__ __forceinline__ void join_pair(const PagedAttnArgs& a, unsigned index
   using E = typename Elem<T>::type;
   constexpr int NG = kJoinThreads / LG;
   __shared__ f32x4 sh_o[NG][LG];
-  __shared__ float sh_l[NG];
+  __shared__ float sh_ml[NG][2];
   const int apart = a.apart, mine = static_cast<int>(index % apart);
   const int head = static_cast<int>(index / apart % a.hkv);
   const Item it = find_item<ROWS, KEYS, true>(a, static_cast<int>(index / apart / a.hkv));
@@ -1020,37 +1020,64 @@ __device__ __forceinline__ void join_pair(const PagedAttnArgs& a, unsigned index
   for (int r0 = 0; r0 < live; r0 += rows_at_once) {
     const int i0 = r0 + grp / per_row, r = i0 * apart + mine;
     f32x4 acc = (f32x4)(0.f);
-    float L = 0.f;
+    float M = kNegInf, L = 0.f;
     if (i0 < live) {
-      float M = kNegInf;
-      for (int s = lg; s < it.splits; s += LG) M = fmaxf(M, ws[s * step + r]);
+      // some splits at a time: all their loads first, then one step of the running maximum
+      constexpr int U = 16;
+      for (int s0 = part; s0 < it.splits; s0 += U * per_row) {
+        float m[U], l[U];
+        f32x4 x[U];
 #pragma unroll
-      for (int d = 1; d < LG; d <<= 1) M = fmaxf(M, __shfl_xor(M, d));
-      if (M == kNegInf) M = 0.f;
-#pragma unroll 8
-      for (int s = part; s < it.splits; s += per_row) {
-        const float* w = ws + s * step;
-        const float f = __builtin_amdgcn_exp2f(w[r] - M);
-        L += f * w[ROWS + r];
-        if (4 * lg < a.d) {
-          const f32x4 x = *reinterpret_cast<const f32x4*>(w + 2 * ROWS + static_cast<size_t>(r) * a.d + 4 * lg);
+        for (int i = 0; i < U; ++i) {
+          m[i] = kNegInf;
+          l[i] = 0.f;
+          x[i] = (f32x4)(0.f);
+          const int s = s0 + i * per_row;
+          if (s < it.splits) {
+            const float* w = ws + s * step;
+            m[i] = w[r];
+            l[i] = w[ROWS + r];
+            if (4 * lg < a.d) x[i] = *reinterpret_cast<const f32x4*>(w + 2 * ROWS + static_cast<size_t>(r) * a.d + 4 * lg);
+          }
+        }
+        float nm = M;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e] += f * x[e];
+        for (int i = 0; i < U; ++i) nm = fmaxf(nm, m[i]);
+        const float base = nm == kNegInf ? 0.f : nm, f = __builtin_amdgcn_exp2f(M - base);
+        M = nm;
+        L *= f;
+        acc *= f;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          const float g = __builtin_amdgcn_exp2f(m[i] - base);
+          L += g * l[i];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] += g * x[i][e];
         }
       }
     }
     if (per_row > 1) {  // (the same in every thread)
       __syncthreads();
       sh_o[grp][lg] = acc;
-      if (lg == 0) sh_l[grp] = L;
+      if (lg == 0) {
+        sh_ml[grp][0] = M;
+        sh_ml[grp][1] = L;
+      }
       __syncthreads();
-      if (part == 0)
+      if (part == 0) {
+        float nm = M;
+        for (int i = 1; i < per_row; ++i) nm = fmaxf(nm, sh_ml[grp + i][0]);
+        const float base = nm == kNegInf ? 0.f : nm, f = __builtin_amdgcn_exp2f(M - base);
+        L *= f;
+        acc *= f;
         for (int i = 1; i < per_row; ++i) {
+          const float g = __builtin_amdgcn_exp2f(sh_ml[grp + i][0] - base);
+          L += g * sh_ml[grp + i][1];
           const f32x4 x = sh_o[grp + i][lg];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e] += x[e];
-          L += sh_l[grp + i];
+          for (int e = 0; e < 4; ++e) acc[e] += g * x[e];
         }
+      }
     }
     if (part != 0 || i0 >= live || 4 * lg >= a.d) continue;
     const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
