@@ -232,7 +232,23 @@ __device__ Item find_item(const PagedAttnArgs& a, int index) {
       const Seq x = seq_of<ROWS, KEYS>(a, b);
       work += static_cast<float>(x.tiles) * static_cast<float>(x.blocks);
     }
-  const int chunk = chunk_of(a, last_lane(wave_scan(work)));
+  int chunk = chunk_of(a, last_lane(wave_scan(work)));
+  // A form that runs one workgroup a compute unit: items just beyond a round
+  // take a whole one more, so of some splits the one with the least rounds times blocks is taken.
+  if (a.one_round > 0 && B1 <= 64) {
+    const int c0 = chunk;
+    int best = 0x7fffffff;
+#pragma unroll
+    for (int x = 4; x <= 16; x += x < 8 ? 1 : 4) {  // 1, 1.25, 1.5, 1.75, 2, 3, 4 times
+      const int c = c0 * x / 4;
+      const int items = last_lane(wave_scan(s.tiles * splits_of(s, c)));
+      const int cost = (items + a.one_round - 1) / a.one_round * c;
+      if (cost < best) {
+        best = cost;
+        chunk = c;
+      }
+    }
+  }
   Count before{0, 0};
   for (int b0 = 0; b0 < B1; b0 += 64) {
     if (b0 > 0) {
@@ -1023,7 +1039,7 @@ __device__ __forceinline__ void join_pair(const PagedAttnArgs& a, unsigned index
     float M = kNegInf, L = 0.f;
     if (i0 < live) {
       // some splits at a time: all their loads first, then one step of the running maximum
-      constexpr int U = 16;
+      constexpr int U = 8;
       for (int s0 = part; s0 < it.splits; s0 += U * per_row) {
         float m[U], l[U];
         f32x4 x[U];
@@ -1143,7 +1159,7 @@ PagedAttnArgs part_of(const PagedAttnArgs& a0, int rows, int rows_lo, int rows_h
   a.min_chunk = min_chunk;
   a.pairs = static_cast<int>(pairs_bound(a, rows));
   a.slots = a.pairs + a.target;
-  a.apart = static_cast<int>(std::clamp<int64_t>(rows / kRows * 4 * kCus / (static_cast<int64_t>(a.pairs) * a.hkv), 1, 32));
+  a.apart = static_cast<int>(std::clamp<int64_t>(rows / kRows * 4 * kCus / (static_cast<int64_t>(a.pairs) * a.hkv), 1, rows > kRows ? rows / 32 : kRows));
   return a;
 }
 
@@ -1179,6 +1195,7 @@ Plan plan_of(PagedAttnArgs a) {
   // The tile form where whole tiles do not fill the card.
   const int64_t tiles = (static_cast<int64_t>(a.p.T) * a.group + tile_rows(a) - 1) / tile_rows(a) * a.hkv;
   p.t = part_of(a, tile_rows(a), p.stream ? kStreamRows : 0, kAllRows, tiles >= 2 * kCus ? 0 : kCus, 4);
+  p.t.one_round = p.t.target;
   p.t.ws = static_cast<char*>(a.ws) + (p.stream ? part_bytes(p.s, kRows) : 0);
   return p;
 }
