@@ -80,9 +80,9 @@ struct RopeArgs {
   void* kc = nullptr;
   void* vc = nullptr;
   int64_t kp = 0, kh = 0, kr = 0, vp = 0, vh = 0, vr = 0;
-  // backward: gradients of the weights (fp32, [d] each, null: not wanted) and their scratch
-  float* dwq = nullptr;
-  float* dwk = nullptr;
+  // backward: gradients of the weights ([d] each in the weights' type, null: not wanted) and their scratch
+  void* dwq = nullptr;
+  void* dwk = nullptr;
   float* ws = nullptr;
 };
 // y = R(position) (w . x / sqrt(mean x^2 + eps)) for every head of q and k; a row

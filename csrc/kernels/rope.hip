@@ -90,6 +90,36 @@ __device__ __forceinline__ void load_piece(const typename T::E* p, float* x) {
   }
 }
 
+// A piece as loaded: several can be under way before the first is unpacked
+template <typename T, int VEC>
+struct Raw {
+  static constexpr int W = VEC * sizeof(typename T::E) / 4;
+  uint32_t w[W];
+  __device__ __forceinline__ void load(const typename T::E* p) {
+    if constexpr (W == 4) {
+      const u32x4 v = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = v[e];
+    } else {
+      const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+      w[0] = v[0];
+      w[1] = v[1];
+    }
+  }
+  __device__ __forceinline__ void unpack(float* x) const {
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      if constexpr (sizeof(typename T::E) == 4) {
+        x[e] = __uint_as_float(w[e]);
+      } else {
+        const f32x2 v = unpack2<T>(w[e]);
+        x[2 * e] = v[0];
+        x[2 * e + 1] = v[1];
+      }
+    }
+  }
+};
+
 template <typename T, int VEC>
 __device__ __forceinline__ void store_piece(typename T::E* p, const float* x) {
   if constexpr (sizeof(typename T::E) == 4) {
@@ -270,19 +300,22 @@ __global__ __launch_bounds__(512) void rope_forward(RopeArgs a) {
 
   const E* xp = static_cast<const E*>(r.x) + b * r.sb + s * r.ss + h * r.sh;
   float x[2 * VEC];
-#pragma unroll
-  for (int i = 0; i < 2 * VEC; ++i) x[i] = 0.f;
+  Raw<T, VEC> xr[2]{};
   if (pos >= 0) {
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-      if (l.has[e]) load_piece<T, VEC>(xp + l.c[e], x + e * VEC);
+      if (l.has[e]) xr[e].load(xp + l.c[e]);
   }
-  if (!is_v && pos >= 0) {
-    float cs[VEC], sn[VEC];
+  float cs[VEC], sn[VEC], w[2 * VEC];
+  const bool turns = !is_v && pos >= 0;
+  if (turns) {  // (every load before the first use)
     load_angles<VEC, INTER>(a.rope == nullptr ? nullptr : a.rope + pos * a.rstride, l, a.rot, cs, sn);
+    if (a.norm) load_weight<T, VEC>(r.w, a.w_f32, l, w);
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) xr[e].unpack(x + e * VEC);
+  if (turns) {
     if (a.norm) {
-      float w[2 * VEC];
-      load_weight<T, VEC>(r.w, a.w_f32, l, w);
       float ss = 0.f;
 #pragma unroll
       for (int i = 0; i < 2 * VEC; ++i) ss += x[i] * x[i];
@@ -325,25 +358,37 @@ __global__ __launch_bounds__(512) void rope_backward(RopeArgs a) {
 #pragma unroll
   for (int i = 0; i < 2 * VEC; ++i) dw[i] = 0.f;
   const int tokens = a.B * a.S;
-  if (live)
+  // A token's rows are loaded while the one before it is worked on
+  Raw<T, VEC> xr[2]{}, gr[2]{};
+  int64_t pos = -1;
+  auto fetch = [&](int t) {
+    if (t >= tokens) return;
+    const int b = t / a.S, s = t - b * a.S;
+    pos = position_of(a, b, s);
+    const E* xp = static_cast<const E*>(r.x) + b * r.sb + s * r.ss + h * r.sh;
+    const E* gp = static_cast<const E*>(r.g) + b * r.gb + s * r.gs + h * r.gh;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (l.has[e]) {
+        xr[e].load(xp + l.c[e]);
+        gr[e].load(gp + l.c[e]);
+      }
+  };
+  if (live) {
+    fetch(blockIdx.x);
     for (int t = blockIdx.x; t < tokens; t += gridDim.x) {
-      const int b = t / a.S, s = t - b * a.S;
-      int64_t pos = position_of(a, b, s);
-      if (pos >= a.positions) pos = -1;
-      float x[2 * VEC], g[2 * VEC];
+      float x[2 * VEC], g[2 * VEC], y[2 * VEC], cs[VEC], sn[VEC];
 #pragma unroll
-      for (int i = 0; i < 2 * VEC; ++i) x[i] = g[i] = 0.f;
-      if (pos >= 0) {
-        const E* xp = static_cast<const E*>(r.x) + b * r.sb + s * r.ss + h * r.sh;
-        const E* gp = static_cast<const E*>(r.g) + b * r.gb + s * r.gs + h * r.gh;
+      for (int e = 0; e < 2; ++e) {
+        xr[e].unpack(x + e * VEC);
+        gr[e].unpack(g + e * VEC);
+      }
+      const bool there = pos >= 0 && pos < a.positions;
+      if (there) load_angles<VEC, INTER>(a.rope + pos * a.rstride, l, a.rot, cs, sn);
+      fetch(t + gridDim.x);
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if (l.has[e]) {
-            load_piece<T, VEC>(xp + l.c[e], x + e * VEC);
-            load_piece<T, VEC>(gp + l.c[e], g + e * VEC);
-          }
-        float cs[VEC], sn[VEC];
-        load_angles<VEC, INTER>(a.rope + pos * a.rstride, l, a.rot, cs, sn);
+      for (int i = 0; i < 2 * VEC; ++i) y[i] = 0.f;
+      if (there) {
         turn<VEC, INTER>(g, cs, sn, -1.f);
         float ss = 0.f, dot = 0.f;
 #pragma unroll
@@ -356,14 +401,15 @@ __global__ __launch_bounds__(512) void rope_backward(RopeArgs a) {
 #pragma unroll
         for (int i = 0; i < 2 * VEC; ++i) {
           dw[i] += g[i] * x[i] * inv;
-          x[i] = inv * (g[i] * w[i] - x[i] * f);
+          y[i] = inv * (g[i] * w[i] - x[i] * f);
         }
       }
       E* yp = static_cast<E*>(r.y) + (static_cast<int64_t>(t) * r.heads + h) * a.d;
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        if (l.has[e]) store_piece<T, VEC>(yp + l.c[e], x + e * VEC);
+        if (l.has[e]) store_piece<T, VEC>(yp + l.c[e], y + e * VEC);
     }
+  }
   if (a.ws == nullptr) return;
 #pragma unroll
   for (int e = 0; e < 2; ++e)
@@ -381,21 +427,36 @@ __global__ __launch_bounds__(512) void rope_backward(RopeArgs a) {
   }
 }
 
-// column sums of the workgroups' partial weight gradients [n][2 d]: a wave takes
-// 16 columns, its four lane groups every fourth row of the wave's share; then the waves in order
-__global__ __launch_bounds__(1024) void rope_dw_sum(const float* ws, int n, int d, float* dwq, float* dwk) {
-  __shared__ float sh[64][16];
-  const int col = blockIdx.x * 16 + (threadIdx.x & 15), row = threadIdx.x >> 4;
+// column sums of the workgroups' partial weight gradients [n][2 d], in the
+// weights' type: a workgroup takes 8 columns, each of its 128 rows of threads
+// every 128th partial sum; then the rows in order
+template <typename T>
+__global__ __launch_bounds__(1024) void rope_dw_sum(const float* ws, int n, int d, typename T::E* dwq, typename T::E* dwk) {
+  __shared__ float sh[128][9], part[16][9];
+  const int c = threadIdx.x & 7, col = blockIdx.x * 8 + c, row = threadIdx.x >> 3;
   float x = 0.f;
-  if (col < 2 * d)
-    for (int i = row; i < n; i += 64) x += ws[static_cast<int64_t>(i) * 2 * d + col];
-  sh[row][threadIdx.x & 15] = x;
+#pragma unroll 16
+  for (int i = row; i < n; i += 128) x += ws[static_cast<int64_t>(i) * 2 * d + col];
+  sh[row][c] = x;
   __syncthreads();
-  if (row != 0 || col >= 2 * d) return;
+  if (row < 16) {
+    x = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x += sh[row * 8 + i][c];
+    part[row][c] = x;
+  }
+  __syncthreads();
+  if (row != 0) return;
   x = 0.f;
-  for (int i = 0; i < 64; ++i) x += sh[i][threadIdx.x];
-  float* out = col < d ? dwq : dwk;
-  if (out != nullptr) out[col < d ? col : col - d] = x;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x += part[i][c];
+  typename T::E* out = col < d ? dwq : dwk;
+  if (out == nullptr) return;
+  out += col < d ? col : col - d;
+  if constexpr (sizeof(typename T::E) == 4)
+    *out = x;
+  else
+    *out = static_cast<uint16_t>(pack2<T>(x, 0.f));
 }
 
 // ---------------------------------------------------------------- launch ----
@@ -510,8 +571,18 @@ void qk_norm_rope_backward(const RopeArgs& a, hipStream_t s) {
       rope_backward<decltype(t), decltype(vec)::value, LPR, decltype(inter)::value>
           <<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(slices)), threads, lds, s>>>(a);
     });
-  if (a.dwq != nullptr || a.dwk != nullptr)
-    rope_dw_sum<<<(2 * a.d + 15) / 16, 1024, 0, s>>>(a.ws, n, a.d, a.dwq, a.dwk);
+  if (a.dwq == nullptr && a.dwk == nullptr) return;
+  auto sum = [&](auto t) {
+    using T = decltype(t);
+    using E = typename T::E;
+    rope_dw_sum<T><<<2 * a.d / 8, 1024, 0, s>>>(a.ws, n, a.d, static_cast<E*>(a.dwq), static_cast<E*>(a.dwk));
+  };
+  if (a.w_f32 || a.type == AttnType::kF32)
+    sum(F32{});
+  else if (a.type == AttnType::kBF16)
+    sum(BF16{});
+  else
+    sum(F16{});
 }
 
 }  // namespace kernels

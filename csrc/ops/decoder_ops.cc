@@ -391,10 +391,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_backward
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(q0.device());
   at::Tensor dq = packed_like(q0), dk = packed_like(k0);
   const auto f32 = q0.options().dtype(at::kFloat);
-  at::Tensor dwq = given(qw) ? at::empty({qw->size(0)}, f32) : at::empty({0}, f32);
-  at::Tensor dwk = given(kw) ? at::empty({kw->size(0)}, f32) : at::empty({0}, f32);
-  auto weights_type = [&](const at::Tensor& dw, const OptTensor& w) { return given(w) ? dw.to(w->scalar_type()) : dw; };
-  if (dq.numel() == 0) return {dq, dk, weights_type(dwq.zero_(), qw), weights_type(dwk.zero_(), kw)};
+  auto like_weight = [&](const OptTensor& w) {
+    return given(w) ? at::empty({w->size(0)}, f32.dtype(w->scalar_type())) : at::empty({0}, f32);
+  };
+  at::Tensor dwq = like_weight(qw), dwk = like_weight(kw);
+  if (dq.numel() == 0) return {dq, dk, dwq.zero_(), dwk.zero_()};
   const at::Tensor q = rows_aligned(q0, row_bytes(q0)), k = rows_aligned(k0, row_bytes(k0));
   const at::Tensor gq = rows_aligned(gq0, row_bytes(q0)), gk = rows_aligned(gk0, row_bytes(k0));
   nnsx::kernels::RopeArgs a;
@@ -408,11 +409,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_backward
   if (given(qw) || given(kw)) {
     ws = at::empty({static_cast<int64_t>(nnsx::kernels::qk_norm_rope_backward_workspace_bytes(a) / sizeof(float))}, f32);
     a.ws = ws.data_ptr<float>();
-    a.dwq = given(qw) ? dwq.data_ptr<float>() : nullptr;
-    a.dwk = given(kw) ? dwk.data_ptr<float>() : nullptr;
+    a.dwq = given(qw) ? dwq.data_ptr() : nullptr;
+    a.dwk = given(kw) ? dwk.data_ptr() : nullptr;
   }
   nnsx::kernels::qk_norm_rope_backward(a, cur_stream());
-  return {dq, dk, weights_type(dwq, qw), weights_type(dwk, kw)};
+  return {dq, dk, dwq, dwk};
 }
 
 // cosines and sines [.., 1, rot / 2] of the tokens, and which rows the table holds
