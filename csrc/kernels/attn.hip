@@ -233,16 +233,17 @@ __device__ Item find_item(const PagedAttnArgs& a, int index) {
       work += static_cast<float>(x.tiles) * static_cast<float>(x.blocks);
     }
   int chunk = chunk_of(a, last_lane(wave_scan(work)));
-  // A form that runs one workgroup a compute unit: items just beyond a round
-  // take a whole one more, so of some splits the one with the least rounds times blocks is taken.
+  // A form of few workgroups a compute unit: items just beyond a round take a
+  // whole one more, and each may have a cost of its own, so of some splits the one with
+  // the least rounds times blocks is taken.
   if (a.one_round > 0 && B1 <= 64) {
     const int c0 = chunk;
     int best = 0x7fffffff;
-#pragma unroll
-    for (int x = 4; x <= 16; x += x < 8 ? 1 : 4) {  // 1, 1.25, 1.5, 1.75, 2, 3, 4 times
-      const int c = c0 * x / 4;
+#pragma unroll 1
+    for (int x = 4; x <= 24; x += x < 6 ? 1 : x < 8 ? 2 : x < 16 ? 4 : 8) {  // 1, 1.25, 1.5, 2, 3, 4, 6 times
+      const int c = static_cast<int>(min(static_cast<int64_t>(c0) * x / 4, static_cast<int64_t>(1 << 24)));
       const int items = last_lane(wave_scan(s.tiles * splits_of(s, c)));
-      const int cost = (items + a.one_round - 1) / a.one_round * c;
+      const int cost = (items + a.one_round - 1) / a.one_round * (c + a.item_cost);
       if (cost < best) {
         best = cost;
         chunk = c;
@@ -453,11 +454,14 @@ __device__ __forceinline__ void stream_item(const PagedAttnArgs& a, unsigned ind
 
   int blk = blk0 + wave;
   KeyRow here = row_of(blk), then = row_of(blk + kWaves);
-  if (blk < blk1) {
+  // (fp32 rows of 256 columns: K and V of a block share registers, nothing is loaded ahead)
+  constexpr bool LOAD_AHEAD = DP * sizeof(E) <= 512;
+  if (LOAD_AHEAD && blk < blk1) {
     load_k(here);
     load_v(here);
   }
   while (blk < blk1) {
+    if (!LOAD_AHEAD) load_k(here);
     const int next = blk + kWaves;
     const int key0 = blk * kKeys;
     const uint32_t there = static_cast<uint32_t>(__ballot(is_there(a, here)));  // (lanes 0 .. 31: the block's keys)
@@ -465,14 +469,19 @@ __device__ __forceinline__ void stream_item(const PagedAttnArgs& a, unsigned ind
     if constexpr (WIDE) {
 #pragma unroll
       for (int i = 0; i < KC; ++i)
+        if (2 * i * PIECE < a.d) {  // (256 cycles)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k[i][e]), __uint_as_float(q_piece(i)[e]), s, 0, 0, 0);
+          for (int e = 0; e < 4; ++e)
+            s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k[i][e]), __uint_as_float(q_piece(i)[e]), s, 0, 0, 0);
+        }
     } else {
 #pragma unroll
       for (int i = 0; i < KC; ++i) s = mfma16<T>(k[i], q_piece(i), s);
     }
-    if (next < blk1) load_k(then);
+    if (!LOAD_AHEAD)
+      load_v(here);
+    else if (next < blk1)
+      load_k(then);
     // every row of the tile sees every key of the block?
     const bool full = there == 0xffffffffu && __all(!live || (rlo <= key0 && key0 + kKeys <= rhi));
     if (!full) {
@@ -565,7 +574,7 @@ __device__ __forceinline__ void stream_item(const PagedAttnArgs& a, unsigned ind
           o[m] = mfma16<T>(vt, p[t], o[m]);
         }
     }
-    if (next < blk1) load_v(then);
+    if (LOAD_AHEAD && next < blk1) load_v(then);
     here = then;
     then = row_of(next + kWaves);
     blk = next;
@@ -1187,7 +1196,11 @@ Plan plan_of(PagedAttnArgs a) {
     p.tile = a.p.B > 1 || static_cast<int64_t>(a.p.T) * a.group > kStreamRows;
   p.stream = !p.tile || a.p.B > 1;
   // The stream form always splits: a sequence much longer than the others is spread over the card.
-  p.s = part_of(a, kRows, 0, p.tile ? kStreamRows : kAllRows, (p.tile ? 2 : 8) * kCus, p.tile ? 8 : 4);
+  p.s = part_of(a, kRows, 0, p.tile ? kStreamRows : kAllRows, (p.tile ? 2 : a.type == AttnType::kF32 ? 3 : 8) * kCus, p.tile ? 8 : 4);
+  if (a.type == AttnType::kF32) {
+    p.s.one_round = ((a.d <= 64 ? 2 : 1) * kCus + a.hkv - 1) / a.hkv;
+    p.s.item_cost = 6;
+  }
   if (p.tile) {  // (two tiles a sequence at most, and the rows behind the last)
     p.s.pairs = static_cast<int>(std::min<int64_t>(p.s.pairs, 2 * (static_cast<int64_t>(a.p.B) + 1)));
     p.s.slots = p.s.pairs + p.s.target;
