@@ -15,8 +15,10 @@
 // per lane, and P^T is already where the second product wants it -- the order
 // of the summed index is free as long as V^T uses the same one (slot j of lane
 // half h = key 16 s + 8 (j / 4) + 4 h + j % 4).  Scores, maxima, sums and O are
-// fp32; P is rounded to the cache's type for the second product (weights in
-// [0, 1], relative error half a step, as the output's own rounding).
+// fp32; for the second product P is rounded to the cache's type, each weight by
+// at most half a step of itself, as the output is: without that the matrix
+// instruction of 16-bit operands could not take it, and two parts a weight would
+// double the second product.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -92,6 +94,10 @@ __device__ __forceinline__ uint32_t finite_part(uint32_t x) {
   if constexpr (std::is_same_v<T, F32>) return f ? 0u : x;
   return x & ~((f >> 15) * 0xffffu);
 }
+// Weights are e^(score - maximum) times 2^kLift: fp16 has no values below 2^-24, and
+// a hundred thousand keys of less weight each are not nothing
+template <typename T>
+constexpr float kLift = std::is_same_v<T, F16> ? 7.f : 0.f;
 // value number e of a word
 template <typename T>
 __device__ __forceinline__ float value_of(uint32_t x, int e);
@@ -498,9 +504,9 @@ __device__ __forceinline__ void stream_item(const PagedAttnArgs& a, unsigned ind
     for (int i = 1; i < 16; ++i) bm = max2(bm, s[i], inf);
     bm = row_max(bm, inf);
     const float nm = fmaxf(mx, bm * c);
-    const float base = nm == kNegInf ? 0.f : nm;  // (a row that has seen nothing yet)
+    const float to = nm == kNegInf ? 0.f : nm, base = to - kLift<T>;  // (a row may have seen nothing yet)
     if (__any(nm > mx)) {
-      const float f = __builtin_amdgcn_exp2f(mx - base);
+      const float f = __builtin_amdgcn_exp2f(mx - to);
       sum *= f;
 #pragma unroll
       for (int m = 0; m < NB; ++m)
@@ -896,7 +902,7 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, unsigned index
     for (int i = 1; i < 15; i += 2) bm = max3(bm, max2(s[0][i], s[1][i], inf), max2(s[0][i + 1], s[1][i + 1], inf));
     const float nm = fmaxf(mx, row_max(max2(bm, max2(s[0][15], s[1][15], inf), inf), inf) * c);
     // the maximum that weights are relative to follows only steps of more than
-    // 2^8: weights stay within [0, 256], far from any type's range, and the
+    // 2^8: weights stay within [0, 2^15], inside every type's range, and the
     // rescale of O is rare
     if (__any(nm > mx + 8.f)) {
       const float f = __builtin_amdgcn_exp2f(mx - (nm == kNegInf ? 0.f : nm));
@@ -908,7 +914,7 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, unsigned index
       mx = nm;
     }
     if (there != ~0ull || key0 < t_in_lo || key0 + kTileKeys > t_in_hi) take_infinite(v, key0, there);
-    const float base = mx == kNegInf ? 0.f : mx;  // (a row that has seen nothing yet)
+    const float base = (mx == kNegInf ? 0.f : mx) - kLift<T>;  // (a row may have seen nothing yet)
     u32x4 p[4];
     auto weigh = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
@@ -1168,7 +1174,8 @@ PagedAttnArgs part_of(const PagedAttnArgs& a0, int rows, int rows_lo, int rows_h
   a.min_chunk = min_chunk;
   a.pairs = static_cast<int>(pairs_bound(a, rows));
   a.slots = a.pairs + a.target;
-  a.apart = static_cast<int>(std::clamp<int64_t>(rows / kRows * 4 * kCus / (static_cast<int64_t>(a.pairs) * a.hkv), 1, rows > kRows ? rows / 32 : kRows));
+  a.apart = static_cast<int>(std::clamp<int64_t>(rows / kRows * 4 * kCus / (static_cast<int64_t>(a.pairs) * a.hkv), 1,
+                                                 rows > kRows ? rows / 32 : kRows));
   return a;
 }
 
@@ -1188,15 +1195,21 @@ struct Plan {
 Plan plan_of(PagedAttnArgs a) {
   a.group = a.hq / a.hkv;
   Plan p;
-  // One token a sequence on average: the stream form takes every sequence.
-  // A single sequence is one form's.  Else both run, each on its own sequences.
-  if (a.type == AttnType::kF32 || a.p.T <= a.p.B)
+  const int64_t rows = static_cast<int64_t>(a.p.T) * a.group;
+  // As many tokens as sequences (single tokens, as a rule) or no more rows than
+  // one tile has: the stream form takes every sequence (64 single tokens: 221 us,
+  // 226 us by both).  A single sequence is one form's: of 64 rows on the tile form is the faster one.
+  // Else both run, each on its own sequences.
+  if (a.type == AttnType::kF32)
     p.tile = false;
+  else if (a.p.B == 1)
+    p.tile = rows > kStreamRows;
   else
-    p.tile = a.p.B > 1 || static_cast<int64_t>(a.p.T) * a.group > kStreamRows;
+    p.tile = a.p.T != a.p.B && rows > tile_rows(a);
   p.stream = !p.tile || a.p.B > 1;
   // The stream form always splits: a sequence much longer than the others is spread over the card.
-  p.s = part_of(a, kRows, 0, p.tile ? kStreamRows : kAllRows, (p.tile ? 2 : a.type == AttnType::kF32 ? 3 : 8) * kCus, p.tile ? 8 : 4);
+  const int per_cu = p.tile ? 2 : a.type == AttnType::kF32 ? 3 : 8;
+  p.s = part_of(a, kRows, 0, p.tile ? kStreamRows : kAllRows, per_cu * kCus, p.tile ? 8 : 4);
   if (a.type == AttnType::kF32) {
     p.s.one_round = ((a.d <= 64 ? 2 : 1) * kCus + a.hkv - 1) / a.hkv;
     p.s.item_cost = 6;
@@ -1206,7 +1219,7 @@ Plan plan_of(PagedAttnArgs a) {
     p.s.slots = p.s.pairs + p.s.target;
   }
   // The tile form where whole tiles do not fill the card.
-  const int64_t tiles = (static_cast<int64_t>(a.p.T) * a.group + tile_rows(a) - 1) / tile_rows(a) * a.hkv;
+  const int64_t tiles = (rows + tile_rows(a) - 1) / tile_rows(a) * a.hkv;
   p.t = part_of(a, tile_rows(a), p.stream ? kStreamRows : 0, kAllRows, tiles >= 2 * kCus ? 0 : kCus, 4);
   p.t.one_round = p.t.target;
   p.t.ws = static_cast<char*>(a.ws) + (p.stream ? part_bytes(p.s, kRows) : 0);

@@ -76,6 +76,9 @@ struct Cache {
   int64_t pages, heads, page, dim;
 };
 
+// (a launch counts its threads in 32 bits: up to 512 of them for a token)
+constexpr int64_t kMaxTokens = (1 << 23) - 1;
+
 Cache check_cache(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& table,
                   const at::Tensor& cu, const at::Tensor& len, const char* op) {
   check_like(k, q, op, "k_cache");
@@ -89,9 +92,9 @@ Cache check_cache(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     bool ok = t->stride(3) == 1 && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0;
     for (int64_t i = 0; i < 3; ++i) ok = ok && (t->size(i) <= 1 || t->stride(i) * t->element_size() % 16 == 0);
     TORCH_CHECK(ok, op, ": rows of the cache start at multiples of 16 bytes and are packed, got strides ", t->strides());
-    for (int64_t i : {0, 2})
-      TORCH_CHECK(t->size(i) <= 1 || (t->stride(i) >= 0 && t->stride(i) * t->element_size() <= (int64_t{1} << 31)), op,
-                  ": pages and rows of the cache are at most 2 GiB apart, got strides ", t->strides());
+    TORCH_CHECK((t->size(0) <= 1 || t->stride(0) * t->element_size() <= (int64_t{1} << 31)) &&
+                    (t->size(2) <= 1 || t->stride(2) * t->element_size() <= (int64_t{1} << 28)),
+                op, ": pages of the cache are at most 2 GiB apart and rows 256 MiB, got strides ", t->strides());
   }
   TORCH_CHECK(table.scalar_type() == at::kInt && table.dim() == 2 && table.device() == q.device() &&
                   (table.size(1) <= 1 || table.stride(1) == 1),
@@ -99,10 +102,12 @@ Cache check_cache(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
               table.scalar_type(), " ", table.sizes(), " on ", table.device());
   check_ints(len, q, table.size(0), op, "kv_lens");
   check_ints(cu, q, table.size(0) + 1, op, "cu_seqlens");
-  constexpr int64_t kMax = std::numeric_limits<int>::max();
-  TORCH_CHECK(c.pages <= kMax && table.size(1) * c.page <= (1 << 30) && q.size(0) * q.size(1) <= (1 << 30) &&
-                  (q.size(0) + table.size(0) + 1) * c.heads * 16 <= kMax,
-              op, ": more tokens, sequences, pages or positions of a sequence than 30 bits count");
+  // (a launch counts its threads in 32 bits: 256 of them for 32 rows, 512 for a sequence)
+  TORCH_CHECK(c.pages <= std::numeric_limits<int>::max() && table.size(1) * c.page <= (1 << 30) &&
+                  q.size(0) <= kMaxTokens && q.size(0) * q.size(1) <= (1 << 27) &&
+                  (table.size(0) + 1) * c.heads <= (1 << 20),
+              op, ": ", q.size(0), " tokens of ", table.size(0), " sequences, tables of ", table.size(1),
+              " pages: more than one call takes");
   return c;
 }
 
@@ -303,9 +308,8 @@ void check_norm(const at::Tensor& q, const at::Tensor& k, const OptTensor& qw, c
   const bool fits = (pos.dim() == 1 && pos.size(0) == q.size(n - 3)) ||
                     (n == 4 && pos.dim() == 2 && pos.size(0) == q.size(0) && pos.size(1) == q.size(1));
   TORCH_CHECK(fits, op, ": positions ", pos.sizes(), " do not fit q ", q.sizes());
-  TORCH_CHECK(q.numel() / q.size(n - 1) <= std::numeric_limits<int>::max() &&
-                  k.numel() / k.size(n - 1) <= std::numeric_limits<int>::max(),
-              op, ": more rows than 31 bits count");
+  TORCH_CHECK(q.numel() / (q.size(n - 1) * q.size(n - 2)) <= kMaxTokens && q.size(n - 2) + k.size(n - 2) <= 65535, op,
+              ": more tokens or heads than one call takes, got q ", q.sizes(), " and k ", k.sizes());
 }
 
 void fill_rows(nnsx::kernels::RopeRows* r, const at::Tensor& x) {
@@ -504,11 +508,12 @@ Cache check_append(const OptTensor& q, const at::Tensor& k, const at::Tensor& v,
               " heads of ", c.dim);
   for (const auto* t : {&k_cache, &v_cache})
     TORCH_CHECK(at::has_internal_overlap(*t) != at::MemOverlap::Yes, op, ": rows of the cache lie on each other");
+  TORCH_CHECK(k_cache.numel() == 0 || k_cache.data_ptr() != v_cache.data_ptr(), op, ": k_cache and v_cache are one");
   if (given(q)) {
     check_like(*q, k, op, "q");
     TORCH_CHECK(q->dim() == 3 && q->size(0) == k.size(0) && q->size(1) > 0 && q->size(2) == c.dim, op, ": q ", q->sizes(),
                 " does not fit k ", k.sizes());
-    TORCH_CHECK(q->size(0) * q->size(1) <= std::numeric_limits<int>::max(), op, ": more rows than 31 bits count");
+    TORCH_CHECK(q->size(1) + 2 * c.heads <= 65535, op, ": more heads than one call takes");
   }
   if (given(rope)) check_rope(*rope, k, c.dim, op);
   TORCH_CHECK(norm || (!given(qw) && !given(kw)), op, ": weights without norm");

@@ -180,6 +180,12 @@ def test_refusals_of_the_cache_and_the_batch(ops):
     refused("no gradient", call, q=s["q"].requires_grad_(True))
     with torch.no_grad():
         call(q=s["q"])
+        far = torch.empty_strided((2, 2, 4, 16), (2 ** 29 + 4, 64, 16, 1))  # (never touched)
+        refused("apart", call, kc=far, vc=far)
+        far = torch.empty_strided((2, 2, 4, 16), (32, 16, 2 ** 26 + 64, 1))
+        refused("apart", call, kc=far, vc=far)
+        refused("more than one call takes", call, q=s["q"][:1].expand(2 ** 23, 4, 16))
+        refused("more than one call takes", call, table=torch.empty_strided((2, 2 ** 28 + 1), (1, 1), dtype=torch.int32))
 
 
 def test_refusals_of_append(ops):
@@ -207,6 +213,7 @@ def test_refusals_of_append(ops):
             s["table"], s["cu"], s["lens"], norm=True, q_weight=w, k_weight=w.half())
     refused("eps", call, norm=True, eps=-1.0)
     refused("lie on each other", call, kc=s["kc"][:1].expand(s["kc"].shape))
+    refused("are one", call, vc=s["kc"])
     refused("no gradient", call, k=s["k"].clone().requires_grad_(True))
 
 
@@ -232,6 +239,7 @@ def test_refusals_of_norm_rope(ops):
     refused("q_weight", call, qw=torch.ones(8))
     refused("k_weight", call, kw=torch.ones(16).half())
     refused("eps", call, eps=float("nan"))
+    refused("more tokens", call, q=q[:1].expand(2 ** 23, 4, 16), k=k[:1].expand(2 ** 23, 2, 16), pos=pos[:1].expand(2 ** 23))
 
 
 def test_script(ops):

@@ -76,6 +76,37 @@ def test_paged_attention_no_sequences(ops):
     assert attend(ops, s).shape == (0, 2, 64)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_paged_attention_empty_slots(ops, dtype):
+    """a batch of fixed slots, most of them empty: prompts among them, as many tokens as slots"""
+    new, kv = [0] * 400, [7] * 400
+    for b, n, m in ((3, 1, 500), (70, 150, 150), (399, 130, 333), (200, 2, 2)):
+        new[b], kv[b] = n, m
+    check(ops, ref.batch(new, kv, 8, 2, 64, 16, dtype, "cuda", pad=1))
+    check(ops, ref.batch([0, 0, 10, 0, 1, 0, 0, 0, 1, 0, 0, 0], [5, 0, 300, 9, 40, 1, 1, 1, 2, 0, 3, 3], 8, 1, 128, 16, dtype, "cuda"))
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_paged_attention_many_small_weights(ops, new):
+    """fp16: a hundred thousand keys whose weights are below fp16's values, beside one of weight 1.
+    They are e^-17.4 = 2.8e-8 each (2^-25 and less is 0 in fp16), together 0.28 % of the sum."""
+    n, page = 100000, 64
+    s = ref.batch([new], [page], 4, 1, 64, page, torch.float16, "cuda")
+    pages = n // page + 1
+    s["kc"] = torch.zeros(pages, 1, page, 64, device="cuda", dtype=torch.float16)
+    s["vc"] = torch.ones_like(s["kc"])
+    s["kc"][0, 0, 0, 0], s["vc"][0, 0, 0] = 1.0, 0.0
+    s["table"] = torch.arange(pages, device="cuda", dtype=torch.int32)[None]
+    s["lens"] = ints(n)
+    s["q"] = torch.zeros(new, 4, 64, device="cuda", dtype=torch.float16)
+    s["q"][..., 0] = 17.4
+    got = attend(ops, s, scale=1.0, causal=False).double()
+    w = (n - 1) * torch.exp(-s["q"][0, 0, 0].double())
+    want = w / (1 + w)
+    # the weights are relative to 2^7 or more: off by at most 2^-12 each; the result by half a step
+    assert (got / want - 1).abs().max() < 2.0 ** -12 + 2.0 ** -11 + 1e-5
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("new", [6, 200])
 def test_paged_attention_hidden_values(ops, dtype, new):
