@@ -205,9 +205,9 @@ __device__ __forceinline__ V last_lane(V x) {
 // key blocks of a split: the items of all pairs stay within `target` more than the pairs
 __device__ __forceinline__ int chunk_of(const PagedAttnArgs& a, float blocks) {
   if (a.target == 0) return 1 << 28;
-  // (a float sum of few terms is off by less than the 1e-4 that is added)
+  // (a float sum of few terms is off by less than the 1e-4 that is added; no sequence has 2^25 blocks)
   const float c = blocks * 1.0001f / static_cast<float>(a.target);
-  return max(static_cast<int>(fminf(c, 2e8f)) + 1, a.min_chunk);
+  return max(static_cast<int>(fminf(c, 33554432.f)) + 1, a.min_chunk);
 }
 
 // pairs, items beyond one a pair << 16 | items of split pairs (both below 2 target)
@@ -227,6 +227,7 @@ __device__ __forceinline__ int splits_of(const Seq& s, int chunk) {
 // sequences at a time; more are summed up first, 64 at a time, by every wave.
 template <int ROWS, int KEYS, bool PAIRS>
 __device__ Item find_item(const PagedAttnArgs& a, int index) {
+#pragma clang fp contract(off)  // (the kernels of a call have to agree on the plan)
   Item it;
   it.b = -1;
   const int lane = threadIdx.x & 63, B1 = a.p.B + 1;
@@ -239,20 +240,32 @@ __device__ Item find_item(const PagedAttnArgs& a, int index) {
       work += static_cast<float>(x.tiles) * static_cast<float>(x.blocks);
     }
   int chunk = chunk_of(a, last_lane(wave_scan(work)));
-  // A form of few workgroups a compute unit: items just beyond a round take a
-  // whole one more, and each may have a cost of its own, so of some splits the one with
-  // the least rounds times blocks is taken.
+  // The card takes `one_round` items of a kv head at once: items just beyond a round take a whole
+  // one more, and each has a cost of its own, so of some splits the one with
+  // the least rounds times blocks is taken (by estimate: sums of reciprocals).
   if (a.one_round > 0 && B1 <= 64) {
     const int c0 = chunk;
-    int best = 0x7fffffff;
-#pragma unroll 1
-    for (int x = 4; x <= 24; x += x < 6 ? 1 : x < 8 ? 2 : x < 16 ? 4 : 8) {  // 1, 1.25, 1.5, 2, 3, 4, 6 times
-      const int c = static_cast<int>(min(static_cast<int64_t>(c0) * x / 4, static_cast<int64_t>(1 << 24)));
-      const int items = last_lane(wave_scan(s.tiles * splits_of(s, c)));
-      const int cost = (items + a.one_round - 1) / a.one_round * (c + a.item_cost);
-      if (cost < best) {
-        best = cost;
-        chunk = c;
+    const int cs[] = {c0, c0 + c0 / 4, c0 + c0 / 2, 2 * c0, 3 * c0, 4 * c0, 6 * c0};
+    const float round = __builtin_amdgcn_rcpf(static_cast<float>(a.one_round));
+    float items[7];
+    auto count = [&](int i) __attribute__((always_inline)) {
+      items[i] = wave_scan(static_cast<float>(s.tiles) *
+                           fmaxf(ceilf(static_cast<float>(s.blocks) * __builtin_amdgcn_rcpf(static_cast<float>(cs[i])) - 1e-3f), 1.f));
+    };
+    auto rounds = [&](int i) __attribute__((always_inline)) { return ceilf(last_lane(items[i]) * round - 1e-3f); };
+    count(0);
+    float least = rounds(0);
+    if (least > 1.f) {
+      least *= static_cast<float>(c0 + a.item_cost);
+#pragma unroll
+      for (int i = 1; i < 7; ++i) count(i);
+#pragma unroll
+      for (int i = 1; i < 7; ++i) {
+        const float cost = rounds(i) * static_cast<float>(cs[i] + a.item_cost);
+        if (cost < least) {
+          least = cost;
+          chunk = cs[i];
+        }
       }
     }
   }
@@ -773,7 +786,9 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, unsigned index
   auto piece_of = [&](int i) { return piece[i % 2]; };  // (the turn repeats every 16 rows, two passes at most)
   static_assert(PASS % 16 == 0 || 2 * PASS % 16 == 0, "tile");
   const int last_page = blk0 < blk1 ? (keys1 - 1) / a.p.page : 0;
-  // ONE_PAGE: the rows of a run share a page; lane i looks after pass i.  Else every lane after its own rows.
+  // ONE_PAGE: the rows of a run share a page; lane i looks after pass i.  Else every lane after its
+  // own rows, of every pass.  (4096 tokens after none, 16 heads of 256 columns, 8 passes: 191 us, 205 us by
+  // the latter; of 128 columns and less, 1 or 2 passes, the latter is as fast and the only one.)
   constexpr int WALKS = ONE_PAGE ? 1 : PASSES;
   int walk_p[WALKS], walk_off[WALKS], id[WALKS], off[WALKS];
   const int dp = kTileKeys / a.p.page, doff = kTileKeys - dp * a.p.page;
@@ -1012,12 +1027,12 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
 }
 
 // A batch of long and short pieces: the tile form's items first, the stream form's after them, one launch.
-template <typename T, int DP, bool ONE_PAGE>
+template <typename T, int DP, bool QUAD>
 __global__ __launch_bounds__(512, 2) void paged_attn_both(PagedAttnArgs t, PagedAttnArgs s, unsigned tiles) {
   if (blockIdx.x < tiles)
-    tile_item<T, DP, 8, ONE_PAGE>(t, blockIdx.x);
+    tile_item<T, DP, 8, false>(t, blockIdx.x);
   else
-    stream_item<T, DP, ONE_PAGE, 8>(s, blockIdx.x - tiles);
+    stream_item<T, DP, QUAD, 8>(s, blockIdx.x - tiles);
 }
 
 // ------------------------------------------------------------------- join ----
@@ -1151,8 +1166,8 @@ void launch_stream(const PagedAttnArgs& a, hipStream_t s) {
 
 template <typename T, int DP, int WAVES>
 void launch_tile(const PagedAttnArgs& a, unsigned grid, hipStream_t s) {
-  if (a.p.page % (512 / DP) == 0)  // (the keys of 1 KiB)
-    paged_attn_tile<T, DP, WAVES, true><<<grid, WAVES * 64, 0, s>>>(a);
+  if (DP > 128 && a.p.page % (512 / DP) == 0)  // (the keys of 1 KiB)
+    paged_attn_tile<T, DP, WAVES, (DP > 128)><<<grid, WAVES * 64, 0, s>>>(a);
   else
     paged_attn_tile<T, DP, WAVES, false><<<grid, WAVES * 64, 0, s>>>(a);
 }
@@ -1166,14 +1181,16 @@ int tile_rows(const PagedAttnArgs& a) { return a.d <= 128 ? 256 : 128; }
 
 // Either form's part of a call: which sequences it takes (by their rows), and
 // how its keys are split: for about `target` items a kv head (0: no split), of at least `min_chunk` key blocks.
-PagedAttnArgs part_of(const PagedAttnArgs& a0, int rows, int rows_lo, int rows_hi, int target, int min_chunk) {
+PagedAttnArgs part_of(const PagedAttnArgs& a0, int rows, int64_t pairs, int rows_lo, int rows_hi, int target, int min_chunk) {
   PagedAttnArgs a = a0;
   a.rows_lo = rows_lo;
   a.rows_hi = rows_hi;
   a.target = (target + a.hkv - 1) / a.hkv;
   a.min_chunk = min_chunk;
-  a.pairs = static_cast<int>(pairs_bound(a, rows));
-  a.slots = a.pairs + a.target;
+  a.pairs = static_cast<int>(pairs);
+  // (no more items than the longest sequence that the tables can hold gives each pair)
+  const int keys = rows == kRows ? kKeys : kTileKeys, blocks = (a.p.width * a.p.page + keys - 1) / keys;
+  a.slots = static_cast<int>(std::min<int64_t>(pairs + a.target, pairs * std::max((blocks + min_chunk - 1) / min_chunk, 1)));
   a.apart = static_cast<int>(std::clamp<int64_t>(rows / kRows * 4 * kCus / (static_cast<int64_t>(a.pairs) * a.hkv), 1,
                                                  rows > kRows ? rows / 32 : kRows));
   return a;
@@ -1185,7 +1202,7 @@ size_t part_bytes(const PagedAttnArgs& a, int rows) {
 
 constexpr int kAllRows = 0x7fffffff;
 // Rows of a sequence up to which the stream form takes it
-constexpr int kStreamRows = 64;
+constexpr int kStreamRows = 32;
 
 struct Plan {
   bool stream, tile;
@@ -1209,18 +1226,13 @@ Plan plan_of(PagedAttnArgs a) {
   p.stream = !p.tile || a.p.B > 1;
   // The stream form always splits: a sequence much longer than the others is spread over the card.
   const int per_cu = p.tile ? 2 : a.type == AttnType::kF32 ? 3 : 8;
-  p.s = part_of(a, kRows, 0, p.tile ? kStreamRows : kAllRows, per_cu * kCus, p.tile ? 8 : 4);
-  if (a.type == AttnType::kF32) {
-    p.s.one_round = ((a.d <= 64 ? 2 : 1) * kCus + a.hkv - 1) / a.hkv;
-    p.s.item_cost = 6;
-  }
-  if (p.tile) {  // (two tiles a sequence at most, and the rows behind the last)
-    p.s.pairs = static_cast<int>(std::min<int64_t>(p.s.pairs, 2 * (static_cast<int64_t>(a.p.B) + 1)));
-    p.s.slots = p.s.pairs + p.s.target;
-  }
+  const int64_t pairs = p.tile ? static_cast<int64_t>(a.p.B) + 1 : pairs_bound(a, kRows);  // (with the tile form: one a sequence)
+  p.s = part_of(a, kRows, pairs, 0, p.tile ? kStreamRows : kAllRows, per_cu * kCus, p.tile ? 8 : 4);
+  p.s.one_round = ((p.tile || (a.type == AttnType::kF32 && a.d > 64) ? 1 : 2) * kCus + a.hkv - 1) / a.hkv;
+  p.s.item_cost = a.type == AttnType::kF32 ? 6 : 16;
   // The tile form where whole tiles do not fill the card.
   const int64_t tiles = (rows + tile_rows(a) - 1) / tile_rows(a) * a.hkv;
-  p.t = part_of(a, tile_rows(a), p.stream ? kStreamRows : 0, kAllRows, tiles >= 2 * kCus ? 0 : kCus, 4);
+  p.t = part_of(a, tile_rows(a), pairs_bound(a, tile_rows(a)), p.stream ? kStreamRows : 0, kAllRows, tiles >= 2 * kCus ? 0 : kCus, 4);
   p.t.one_round = p.t.target;
   p.t.ws = static_cast<char*>(a.ws) + (p.stream ? part_bytes(p.s, kRows) : 0);
   return p;
@@ -1246,7 +1258,7 @@ void launch_join(const Plan& p, hipStream_t s) {
 template <typename T, int DP>
 void launch_both(const Plan& p, hipStream_t s) {
   const unsigned tiles = grid_of(p.t), grid = tiles + grid_of(p.s);
-  if (p.t.p.page % (512 / DP) == 0)
+  if (p.t.p.page % 4 == 0)
     paged_attn_both<T, DP, true><<<grid, 512, 0, s>>>(p.t, p.s, tiles);
   else
     paged_attn_both<T, DP, false><<<grid, 512, 0, s>>>(p.t, p.s, tiles);
