@@ -197,6 +197,21 @@ __device__ __forceinline__ V wave_scan(V x) {
   x += shifted(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
   return x;
 }
+// the least of all lanes, in the last one
+__device__ __forceinline__ float wave_least(float x) {
+  auto other = [&](auto ctrl, auto rows) {  // (where there is none: itself)
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, x), __builtin_bit_cast(int, x),
+                                                                 decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  x = fminf(x, other(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{}));
+  x = fminf(x, other(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{}));
+  x = fminf(x, other(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{}));
+  x = fminf(x, other(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{}));
+  x = fminf(x, other(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{}));
+  x = fminf(x, other(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{}));
+  return x;
+}
 template <typename V>
 __device__ __forceinline__ V last_lane(V x) {
   return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
@@ -241,32 +256,24 @@ __device__ Item find_item(const PagedAttnArgs& a, int index) {
     }
   int chunk = chunk_of(a, last_lane(wave_scan(work)));
   // The card takes `one_round` items of a kv head at once: items just beyond a round take a whole
-  // one more, and each has a cost of its own, so of some splits the one with
-  // the least rounds times blocks is taken (by estimate: sums of reciprocals).
-  if (a.one_round > 0 && B1 <= 64) {
-    const int c0 = chunk;
-    const int cs[] = {c0, c0 + c0 / 4, c0 + c0 / 2, 2 * c0, 3 * c0, 4 * c0, 6 * c0};
+  // one more, and each has a cost of its own.  If it is more than a round, of the splits 1, 1 1/8, .. 8 7/8
+  // times as long, one a lane, the one with the least rounds times blocks is taken (by
+  // estimate: products with reciprocals).
+  if (a.target > 0 && B1 <= 64) {  // (chunk < 2^26)
     const float round = __builtin_amdgcn_rcpf(static_cast<float>(a.one_round));
-    float items[7];
-    auto count = [&](int i) __attribute__((always_inline)) {
-      items[i] = wave_scan(static_cast<float>(s.tiles) *
-                           fmaxf(ceilf(static_cast<float>(s.blocks) * __builtin_amdgcn_rcpf(static_cast<float>(cs[i])) - 1e-3f), 1.f));
+    auto splits = [&](int tiles, int blocks, float of) __attribute__((always_inline)) {
+      return static_cast<float>(tiles) * fmaxf(ceilf(static_cast<float>(blocks) * of - 1e-3f), 1.f);
     };
-    auto rounds = [&](int i) __attribute__((always_inline)) { return ceilf(last_lane(items[i]) * round - 1e-3f); };
-    count(0);
-    float least = rounds(0);
-    if (least > 1.f) {
-      least *= static_cast<float>(c0 + a.item_cost);
-#pragma unroll
-      for (int i = 1; i < 7; ++i) count(i);
-#pragma unroll
-      for (int i = 1; i < 7; ++i) {
-        const float cost = rounds(i) * static_cast<float>(cs[i] + a.item_cost);
-        if (cost < least) {
-          least = cost;
-          chunk = cs[i];
-        }
+    if (last_lane(wave_scan(splits(s.tiles, s.blocks, __builtin_amdgcn_rcpf(static_cast<float>(chunk))))) * round > 1.001f) {
+      const int c = chunk + chunk / 8 * lane + chunk % 8 * lane / 8;
+      const float of = __builtin_amdgcn_rcpf(static_cast<float>(c));
+      float items = 0.f;
+      for (uint64_t left = __ballot(s.tiles > 0); left != 0; left &= left - 1) {
+        const int l = __builtin_ctzll(left);
+        items += splits(__builtin_amdgcn_readlane(s.tiles, l), __builtin_amdgcn_readlane(s.blocks, l), of);
       }
+      const float cost = ceilf(items * round - 1e-3f) * static_cast<float>(c + a.item_cost);
+      chunk = __builtin_amdgcn_readlane(c, __builtin_ctzll(__ballot(cost == last_lane(wave_least(cost)))));
     }
   }
   Count before{0, 0};
@@ -918,7 +925,7 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, unsigned index
     const float nm = fmaxf(mx, row_max(max2(bm, max2(s[0][15], s[1][15], inf), inf), inf) * c);
     // the maximum that weights are relative to follows only steps of more than
     // 2^8: weights stay within [0, 2^15], inside every type's range, and the
-    // rescale of O is rare
+    // rescale of O is rare (8192 tokens, 32 heads of 128 columns: 580 us, 605 us with every step followed)
     if (__any(nm > mx + 8.f)) {
       const float f = __builtin_amdgcn_exp2f(mx - (nm == kNegInf ? 0.f : nm));
       sum *= f;
@@ -1145,6 +1152,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_attn_join(PagedAttnArgs t,
   join_pair<T, kRows, kKeys, LG>(s, blockIdx.x - tiles);
 }
 
+// (60 tokens after 8192, 8 heads of 128 columns: 371 us, 394 us with every row of V addressed by itself)
 template <typename T, int DP>
 void launch_stream(const PagedAttnArgs& a, unsigned grid, hipStream_t s) {
   if (a.p.page % 4 == 0)
@@ -1183,14 +1191,15 @@ int tile_rows(const PagedAttnArgs& a) { return a.d <= 128 ? 256 : 128; }
 // how its keys are split: for about `target` items a kv head (0: no split), of at least `min_chunk` key blocks.
 PagedAttnArgs part_of(const PagedAttnArgs& a0, int rows, int64_t pairs, int rows_lo, int rows_hi, int target, int min_chunk) {
   PagedAttnArgs a = a0;
-  a.rows_lo = rows_lo;
-  a.rows_hi = rows_hi;
-  a.target = (target + a.hkv - 1) / a.hkv;
-  a.min_chunk = min_chunk;
-  a.pairs = static_cast<int>(pairs);
   // (no more items than the longest sequence that the tables can hold gives each pair)
   const int keys = rows == kRows ? kKeys : kTileKeys, blocks = (a.p.width * a.p.page + keys - 1) / keys;
-  a.slots = static_cast<int>(std::min<int64_t>(pairs + a.target, pairs * std::max((blocks + min_chunk - 1) / min_chunk, 1)));
+  const int most = std::max((blocks + min_chunk - 1) / min_chunk, 1);
+  a.rows_lo = rows_lo;
+  a.rows_hi = rows_hi;
+  a.target = most > 1 ? (target + a.hkv - 1) / a.hkv : 0;
+  a.min_chunk = min_chunk;
+  a.pairs = static_cast<int>(pairs);
+  a.slots = static_cast<int>(std::min<int64_t>(pairs + a.target, pairs * most));
   a.apart = static_cast<int>(std::clamp<int64_t>(rows / kRows * 4 * kCus / (static_cast<int64_t>(a.pairs) * a.hkv), 1,
                                                  rows > kRows ? rows / 32 : kRows));
   return a;
@@ -1201,7 +1210,8 @@ size_t part_bytes(const PagedAttnArgs& a, int rows) {
 }
 
 constexpr int kAllRows = 0x7fffffff;
-// Rows of a sequence up to which the stream form takes it
+// Rows of a sequence up to which the stream form takes it: one item's.  (30 x 16 tokens, 64 rows, beside 2 x 1024,
+// all after 4096: 289 us; 397 us if the stream form takes them, which then reads each key twice.)
 constexpr int kStreamRows = 32;
 
 struct Plan {
@@ -1213,10 +1223,12 @@ Plan plan_of(PagedAttnArgs a) {
   a.group = a.hq / a.hkv;
   Plan p;
   const int64_t rows = static_cast<int64_t>(a.p.T) * a.group;
-  // As many tokens as sequences (single tokens, as a rule) or no more rows than
-  // one tile has: the stream form takes every sequence (64 single tokens: 221 us,
-  // 226 us by both).  A single sequence is one form's: of 64 rows on the tile form is the faster one.
-  // Else both run, each on its own sequences.
+  // Measured with 32 query and 8 kv heads of 128 columns (rows = 4 times the tokens), us.
+  // One sequence: up to 32 rows the stream form (8 tokens after 65536: 54, tile form 79), beyond the
+  // tile form (9 tokens: 81, stream form 80; 32 tokens: 96, 180).
+  // Several: as many tokens as sequences (single tokens, as a rule), or no more rows than one tile has:
+  // the stream form takes all (8 single tokens after 4096: 34, 40 by both; 2 x 16 tokens
+  // after 8192: 33, 37).  Else both run, each on its own sequences (8 x 16 tokens after 4096: 58, stream form 71).
   if (a.type == AttnType::kF32)
     p.tile = false;
   else if (a.p.B == 1)
@@ -1224,16 +1236,24 @@ Plan plan_of(PagedAttnArgs a) {
   else
     p.tile = a.p.T != a.p.B && rows > tile_rows(a);
   p.stream = !p.tile || a.p.B > 1;
-  // The stream form always splits: a sequence much longer than the others is spread over the card.
+  // The stream form always splits: a sequence much longer than the others is spread over the card.  Up to
+  // 8 items a compute unit, where its workgroups are alone (60 single tokens after 8192: 362 us, from 2 a unit on 516 us, as
+  // 480 items are nearly a round already), of which the rounds decide (8 tokens after 4096: 35 us, always 8 a unit 48 us;
+  // 1 after 131072: 105 us and 125 us; 24 after 2048 to 16384, 4 heads: 102 us and 112 us).
   const int per_cu = p.tile ? 2 : a.type == AttnType::kF32 ? 3 : 8;
   const int64_t pairs = p.tile ? static_cast<int64_t>(a.p.B) + 1 : pairs_bound(a, kRows);  // (with the tile form: one a sequence)
   p.s = part_of(a, kRows, pairs, 0, p.tile ? kStreamRows : kAllRows, per_cu * kCus, p.tile ? 8 : 4);
   p.s.one_round = ((p.tile || (a.type == AttnType::kF32 && a.d > 64) ? 1 : 2) * kCus + a.hkv - 1) / a.hkv;
   p.s.item_cost = a.type == AttnType::kF32 ? 6 : 16;
-  // The tile form where whole tiles do not fill the card.
+  // The tile form splits where whole tiles do not fill the card (1300 tokens after 8192, 168 tiles: 212 us,
+  // 317 us whole; 3600 tokens after 16384, 456 tiles: 852 us, 1065 us if those split too: a
+  // split's rows go through memory twice).  Splits of less than 8 blocks cost more than they give
+  // (4 x 100 tokens alone: 25.7 us, 29.1 us with splits of 4).
   const int64_t tiles = (rows + tile_rows(a) - 1) / tile_rows(a) * a.hkv;
-  p.t = part_of(a, tile_rows(a), pairs_bound(a, tile_rows(a)), p.stream ? kStreamRows : 0, kAllRows, tiles >= 2 * kCus ? 0 : kCus, 4);
-  p.t.one_round = p.t.target;
+  p.t = part_of(a, tile_rows(a), pairs_bound(a, tile_rows(a)), p.stream ? kStreamRows : 0, kAllRows,
+                tiles >= kCus ? 0 : 2 * kCus, 8);
+  p.t.one_round = (kCus + a.hkv - 1) / a.hkv;
+  p.t.item_cost = 8;
   p.t.ws = static_cast<char*>(a.ws) + (p.stream ? part_bytes(p.s, kRows) : 0);
   return p;
 }

@@ -76,6 +76,20 @@ def test_paged_attention_no_sequences(ops):
     assert attend(ops, s).shape == (0, 2, 64)
 
 
+def test_paged_attention_more_tiles_than_the_card(ops):
+    """so many rows that no tile's keys are split, and more than one round of them"""
+    check(ops, ref.batch([2100], [2100], 32, 32, 64, 16, torch.bfloat16, "cuda"))
+    check(ops, ref.batch([1000, 5, 1100], [1000, 50, 1500], 32, 32, 64, 16, torch.bfloat16, "cuda"))
+
+
+@pytest.mark.parametrize("lens", [[3000, 2000, 100], [70000], [1] * 62 + [9000], [9000] + [1] * 200 + [300], [517] * 40])
+@pytest.mark.parametrize("new", [1, 8, 33])
+def test_paged_attention_many_splits(ops, lens, new):
+    """more splits than the card takes at once, lengths far apart, more than 64 sequences"""
+    kv = [max(n, new) for n in lens]
+    check(ops, ref.batch([new] * len(kv), kv, 8, 2, 64, 16, torch.bfloat16, "cuda", pad=2))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_paged_attention_empty_slots(ops, dtype):
     """a batch of fixed slots, most of them empty: prompts among them, as many tokens as slots"""
