@@ -103,7 +103,7 @@ Cache check_cache(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
   check_ints(len, q, table.size(0), op, "kv_lens");
   check_ints(cu, q, table.size(0) + 1, op, "cu_seqlens");
   // (a launch counts its threads in 32 bits: 256 of them for 32 rows, 512 for a sequence)
-  TORCH_CHECK(c.pages <= std::numeric_limits<int>::max() && table.size(1) * c.page <= (1 << 30) &&
+  TORCH_CHECK(c.pages <= std::numeric_limits<int>::max() && c.page <= (1 << 30) && table.size(1) <= (1 << 30) / c.page &&
                   q.size(0) <= kMaxTokens && q.size(0) * q.size(1) <= (1 << 27) &&
                   (table.size(0) + 1) * c.heads <= (1 << 20),
               op, ": ", q.size(0), " tokens of ", table.size(0), " sequences, tables of ", table.size(1),
@@ -495,6 +495,17 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_backward
 }
 
 // ---------------------------------------------------------- paged_append ----
+// do the memory ranges of two tensors meet?
+bool meets(const at::Tensor& a, const at::Tensor& b) {
+  auto end = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return static_cast<const char*>(t.data_ptr()) + (last + 1) * t.element_size();
+  };
+  return a.numel() > 0 && b.numel() > 0 && static_cast<const char*>(a.data_ptr()) < end(b) &&
+         static_cast<const char*>(b.data_ptr()) < end(a);
+}
+
 Cache check_append(const OptTensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache,
                    const at::Tensor& v_cache, const at::Tensor& table, const at::Tensor& cu, const at::Tensor& len,
                    const OptTensor& rope, bool norm, const OptTensor& qw, const OptTensor& kw, double eps) {
@@ -508,7 +519,12 @@ Cache check_append(const OptTensor& q, const at::Tensor& k, const at::Tensor& v,
               " heads of ", c.dim);
   for (const auto* t : {&k_cache, &v_cache})
     TORCH_CHECK(at::has_internal_overlap(*t) != at::MemOverlap::Yes, op, ": rows of the cache lie on each other");
-  TORCH_CHECK(k_cache.numel() == 0 || k_cache.data_ptr() != v_cache.data_ptr(), op, ": k_cache and v_cache are one");
+  const auto both = at::get_overlap_status(k_cache, v_cache);
+  TORCH_CHECK((k_cache.numel() == 0 || k_cache.data_ptr() != v_cache.data_ptr()) && both != at::MemOverlapStatus::Full &&
+                  both != at::MemOverlapStatus::Partial,
+              op, ": k_cache and v_cache are one");
+  for (const at::Tensor* t : {&k, &v, given(q) ? &*q : &k})
+    TORCH_CHECK(!meets(*t, k_cache) && !meets(*t, v_cache), op, ": the new rows are a part of the cache");
   if (given(q)) {
     check_like(*q, k, op, "q");
     TORCH_CHECK(q->dim() == 3 && q->size(0) == k.size(0) && q->size(1) > 0 && q->size(2) == c.dim, op, ": q ", q->sizes(),
@@ -641,6 +657,7 @@ class QkNormRope : public torch::autograd::Function<QkNormRope> {
 std::tuple<at::Tensor, at::Tensor> qk_norm_rope_autograd(const at::Tensor& q, const at::Tensor& k, const OptTensor& qw,
                                                          const OptTensor& kw, const at::Tensor& pos,
                                                          const at::Tensor& rope, double eps, bool interleaved) {
+  TORCH_CHECK(!at::GradMode::is_enabled() || !rope.requires_grad(), "qk_norm_rope: no gradient for the table of angles");
   auto y = QkNormRope::apply(q, k, qw, kw, pos, rope, eps, interleaved);
   return {y[0], y[1]};
 }
@@ -675,18 +692,37 @@ at::Tensor paged_attention_autograd(const at::Tensor& q, const at::Tensor& k, co
   return op.call(q, k, v, table, cu, len, scale, causal, window);
 }
 
+const auto& append_op() {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("nnsx::paged_append", "")
+                             .typed<decltype(paged_append_cpu)>();
+  return op;
+}
+
 at::Tensor paged_append_autograd(const OptTensor& q, const at::Tensor& k, const at::Tensor& v, at::Tensor& k_cache,
                                  at::Tensor& v_cache, const at::Tensor& table, const at::Tensor& cu, const at::Tensor& len,
                                  const OptTensor& rope, bool norm, const OptTensor& qw, const OptTensor& kw, double eps,
                                  bool interleaved) {
   const at::Tensor none;
   no_gradient("paged_append", {given(q) ? &*q : &none, &k, &v, &k_cache, &v_cache, given(qw) ? &*qw : &none,
-                               given(kw) ? &*kw : &none});
-  at::AutoDispatchBelowADInplaceOrView below;
-  static const auto op = c10::Dispatcher::singleton()
-                             .findSchemaOrThrow("nnsx::paged_append", "")
-                             .typed<decltype(paged_append_cpu)>();
-  return op.call(q, k, v, k_cache, v_cache, table, cu, len, rope, norm, qw, kw, eps, interleaved);
+                               given(kw) ? &*kw : &none, given(rope) ? &*rope : &none});
+  at::AutoDispatchBelowAutograd below;
+  return append_op().call(q, k, v, k_cache, v_cache, table, cu, len, rope, norm, qw, kw, eps, interleaved);
+}
+
+// what an earlier operation keeps of the cache for its gradient has changed
+at::Tensor paged_append_inplace(const OptTensor& q, const at::Tensor& k, const at::Tensor& v, at::Tensor& k_cache,
+                                at::Tensor& v_cache, const at::Tensor& table, const at::Tensor& cu, const at::Tensor& len,
+                                const OptTensor& rope, bool norm, const OptTensor& qw, const OptTensor& kw, double eps,
+                                bool interleaved) {
+  at::Tensor out;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    out = append_op().call(q, k, v, k_cache, v_cache, table, cu, len, rope, norm, qw, kw, eps, interleaved);
+  }
+  torch::autograd::impl::bump_version(k_cache);
+  torch::autograd::impl::bump_version(v_cache);
+  return out;
 }
 
 }  // namespace
@@ -724,3 +760,5 @@ TORCH_LIBRARY_IMPL(nnsx, Autograd, m) {
   m.impl("paged_append", paged_append_autograd);
   m.impl("paged_attention", paged_attention_autograd);
 }
+
+TORCH_LIBRARY_IMPL(nnsx, ADInplaceOrView, m) { m.impl("paged_append", paged_append_inplace); }

@@ -185,6 +185,8 @@ def test_refusals_of_the_cache_and_the_batch(ops):
         far = torch.empty_strided((2, 2, 4, 16), (32, 16, 2 ** 26 + 64, 1))
         refused("apart", call, kc=far, vc=far)
         refused("more than one call takes", call, q=s["q"][:1].expand(2 ** 23, 4, 16))
+        empty = torch.empty(0, 2, 2 ** 31 + 4, 16)
+        refused("more than one call takes", call, kc=empty, vc=empty, table=torch.empty(2, 0, dtype=torch.int32))
         refused("more than one call takes", call, table=torch.empty_strided((2, 2 ** 28 + 1), (1, 1), dtype=torch.int32))
 
 
@@ -214,7 +216,26 @@ def test_refusals_of_append(ops):
     refused("eps", call, norm=True, eps=-1.0)
     refused("lie on each other", call, kc=s["kc"][:1].expand(s["kc"].shape))
     refused("are one", call, vc=s["kc"])
+    pool = torch.zeros(s["kc"].numel() * 2)
+    part = pool[:s["kc"].numel()].view(s["kc"].shape)
+    refused("are one", call, kc=part, vc=pool[8:8 + s["kc"].numel()].view(s["kc"].shape))
+    refused("part of the cache", call, kc=part, vc=pool[s["kc"].numel():].view(s["kc"].shape), k=pool[:s["k"].numel()].view(s["k"].shape))
+    call(kc=part, vc=pool[s["kc"].numel():].view(s["kc"].shape))
     refused("no gradient", call, k=s["k"].clone().requires_grad_(True))
+    refused("no gradient", call, rope=rope.clone().requires_grad_(True))
+
+
+def test_append_is_seen_by_gradients(ops):
+    """a cache that an earlier operation keeps for its gradient is not changed unnoticed"""
+    s = ref.batch([2, 1], [5, 9], 4, 2, 16, 4, torch.float32)
+    w = torch.ones(16, requires_grad=True)
+    loss = (s["kc"] * w).sum()
+    ops.paged_append(None, s["k"], s["v"], s["kc"], s["vc"], s["table"], s["cu"], s["lens"])
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
+    with torch.inference_mode():
+        s = ref.batch([2, 1], [5, 9], 4, 2, 16, 4, torch.float32)
+        ops.paged_append(None, s["k"], s["v"], s["kc"], s["vc"], s["table"], s["cu"], s["lens"])
 
 
 def test_refusals_of_norm_rope(ops):
@@ -238,6 +259,7 @@ def test_refusals_of_norm_rope(ops):
     refused("positions", call, pos=pos[None])
     refused("q_weight", call, qw=torch.ones(8))
     refused("k_weight", call, kw=torch.ones(16).half())
+    refused("no gradient", call, rope=rope.clone().requires_grad_(True))
     refused("eps", call, eps=float("nan"))
     refused("more tokens", call, q=q[:1].expand(2 ** 23, 4, 16), k=k[:1].expand(2 ** 23, 2, 16), pos=pos[:1].expand(2 ** 23))
 
