@@ -170,9 +170,9 @@ def attention(q, kc, vc, table, cu, lens, scale=None, causal=True, window=0):
                 rel = 2 * e + 2 * (len(keys) + 16) * F32 + (half_step(dtype) if dtype != torch.float32 else 0.0)
                 out[t0:t1, h * group + g] = o
                 tol[t0:t1, h * group + g] = a * rel * 1.01 + o.abs() * half_step(dtype) + smallest(dtype)
-    # (weights below fp16's normal range are off by half a step of 2^-24 each, of a largest weight of 1)
+    # (weights below fp16's normal range are off by half a step of 2^-24 each, of a largest weight of 2^7)
     if dtype == torch.float16:
-        tol = tol + max(lens + [0]) * 2.0 ** -25 * max(1.0, float(vc[vc.isfinite()].abs().max()) if vc.isfinite().any() else 1.0)
+        tol = tol + max(lens + [0]) * 2.0 ** -32 * max(1.0, float(vc[vc.isfinite()].abs().max()) if vc.isfinite().any() else 1.0)
     return out, tol
 
 

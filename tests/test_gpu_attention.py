@@ -78,8 +78,8 @@ def test_paged_attention_no_sequences(ops):
 
 def test_paged_attention_more_tiles_than_the_card(ops):
     """so many rows that no tile's keys are split, and more than one round of them"""
-    check(ops, ref.batch([2100], [2100], 32, 32, 64, 16, torch.bfloat16, "cuda"))
-    check(ops, ref.batch([1000, 5, 1100], [1000, 50, 1500], 32, 32, 64, 16, torch.bfloat16, "cuda"))
+    check(ops, ref.batch([300], [900], 160, 160, 64, 16, torch.bfloat16, "cuda"))
+    check(ops, ref.batch([200, 5, 300], [200, 50, 700], 160, 160, 64, 16, torch.bfloat16, "cuda"))
 
 
 @pytest.mark.parametrize("lens", [[3000, 2000, 100], [70000], [1] * 62 + [9000], [9000] + [1] * 200 + [300], [517] * 40])
@@ -152,6 +152,36 @@ def test_paged_attention_length_behind_the_table(ops, dtype):
     s = ref.batch([1, 70], [64, 70], 4, 2, 64, 16, dtype, "cuda")
     s["table"] = s["table"][:, :3].contiguous()
     check(ops, s)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [1, 2, 3, 4, 12, 100])
+def test_paged_attention_pages(ops, dim, page):
+    """pages of any size in a batch that both forms share, rows behind the last sequence"""
+    s = ref.batch([70, 1, 40, 3], [300, 200, 40, 133], 8, 2, dim, page, torch.bfloat16, "cuda", pad=30)
+    got = check(ops, s)
+    assert (got[114:] == 0).all()
+    s = ref.batch([70], [300], 8, 2, dim, page, torch.float16, "cuda", pad=3)
+    check(ops, s, window=90)
+
+
+@pytest.mark.parametrize("new", [[1, 1], [80, 80], [1, 80]])
+def test_paged_attention_shared_pages(ops, new):
+    """sequences that share their pages: one table row for both"""
+    s = ref.batch([80], [200], 8, 2, 128, 16, torch.bfloat16, "cuda")
+    t = sum(new)
+    s.update(table=s["table"].expand(2, -1), cu=ints(0, new[0], t), lens=ints(200, 190),
+             q=torch.randn(t, 8, 128, device="cuda").bfloat16())
+    got = check(ops, s)
+    assert torch.equal(got, attend(ops, {**s, "table": s["table"].contiguous()}))
+
+
+@pytest.mark.parametrize("new", [1, 120])
+def test_paged_attention_wide_window(ops, new):
+    s = ref.batch([new, 1], [130, 77], 4, 1, 64, 16, torch.bfloat16, "cuda")
+    want = attend(ops, s)
+    for window in (130, 2 ** 30 - 1, 2 ** 30, 2 ** 31, 2 ** 62):
+        assert torch.equal(attend(ops, s, window=window), want), window
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -440,6 +470,27 @@ def test_two_graphs_and_an_eager_stream(ops):
         for o, e, w in zip(outs, eager, want):
             assert torch.equal(o, w) and torch.equal(e, w)
             o.zero_()
+
+
+def test_captured_batches_of_any_kind(ops):
+    """one graph for a number of tokens: single tokens, chunks and prompts among them from replay to replay"""
+    kinds = [([120, 1, 1, 6], [400, 900, 33, 6]), ([1, 1, 1, 125], [100, 1, 500, 125]), ([32, 32, 32, 32], [900, 32, 70, 500]),
+             ([0, 128, 0, 0], [5, 777, 0, 0]), ([1, 1, 1, 1], [900, 20, 300, 5]), ([0, 0, 0, 0], [0, 0, 0, 0])]
+    s = ref.batch([32] * 4, [900] * 4, 8, 2, 128, 16, torch.bfloat16, "cuda")
+    graph = torch.cuda.CUDAGraph()
+    attend(ops, s)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = attend(ops, s)
+    for new, kv in kinds + kinds[::-1]:
+        s["cu"].copy_(ints(0, *torch.tensor(new).cumsum(0).tolist()))
+        s["lens"].copy_(ints(*kv))
+        graph.replay()
+        want = attend(ops, {**s, "cu": s["cu"].clone(), "lens": s["lens"].clone()})
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), new
+        check(ops, s)
+        out.fill_(7.0)
 
 
 def test_captured_gradient(ops):
