@@ -97,6 +97,29 @@ std::string host_h2d(int dev, bool pinned) {
   return r;
 }
 
+// A stream whose work does not hold up `rs`: streams share a few hardware
+// queues, and a free ordered on rs would come after the spin of a stream in its
+// queue whatever it waits for.  Those tried before stay in `tried`, so that the next gets another queue.
+hipStream_t stream_beside(hipStream_t rs, int dev, std::vector<hipStream_t>* tried) {
+  hipEvent_t e = hip::event_get(dev);
+  hipStream_t s = nullptr;
+  for (int i = 0; i < 8; ++i) {
+    hip::check(hipStreamCreateWithFlags(&s, hipStreamNonBlocking), "selftest stream");
+    tried->push_back(s);
+    kernels::spin_us(s, 1);  // (its code is loaded)
+    hip::check(hipStreamSynchronize(s), "selftest sync");
+    kernels::spin_us(s, 4000);
+    hip::check(hipEventRecord(e, rs), "selftest event");
+    std::this_thread::sleep_for(std::chrono::milliseconds(1));
+    const bool passed = hipEventQuery(e) == hipSuccess && hipStreamQuery(s) != hipSuccess;
+    hip::check(hipStreamSynchronize(s), "selftest sync");
+    if (passed) break;
+  }
+  hip::check(hipStreamSynchronize(rs), "selftest sync");
+  hip::event_put(dev, e);
+  return s;
+}
+
 // the mirror of a host memory is read on a second stream (spinning first),
 // which records its use on the HOST memory (what a filter's replay lane does);
 // the host memory and so its mirror are released; a new device block of the
@@ -108,9 +131,10 @@ std::string mirror_other_stream(int dev) {
   // free past the reader and hide the undone fix
   Memory::drain_deferred();
   hip::check(hipStreamSynchronize(hip::release_stream(dev)), "selftest sync");
-  hipStream_t s1 = nullptr, s2 = nullptr;
+  hipStream_t s1 = nullptr;
   hip::check(hipStreamCreateWithFlags(&s1, hipStreamNonBlocking), "selftest stream");
-  hip::check(hipStreamCreateWithFlags(&s2, hipStreamNonBlocking), "selftest stream");
+  std::vector<hipStream_t> tried;
+  hipStream_t s2 = stream_beside(hip::release_stream(dev), dev, &tried);
   // (pageable: its release does not wait for readers on the host -- the mirror's
   // own release must order itself after them)
   MemoryPtr h = Memory::alloc_host(kBytes);
@@ -159,7 +183,7 @@ std::string mirror_other_stream(int dev) {
   out.reset();
   hip::check(hipDeviceSynchronize(), "selftest sync");
   (void)hipStreamDestroy(s1);
-  (void)hipStreamDestroy(s2);
+  for (hipStream_t s : tried) (void)hipStreamDestroy(s);
   return r;
 }
 
