@@ -40,7 +40,7 @@ struct PagedAttnArgs {
   int causal = 1;
   int window = 0;       // 0: no window; else keys in (position - window, position]
   void* ws = nullptr;   // paged_attn_workspace_bytes(a)
-  // derived by the launcher
+  // derived by the launcher: rows a token, and how the keys are split (attn.hip, plan)
   int group = 1, target = 0, min_chunk = 1, slots = 0, pairs = 0, apart = 1, one_round = 0, item_cost = 0, rows_lo = 0, rows_hi = 0;
 };
 // bytes of scratch memory the call needs (0: none)
@@ -48,10 +48,9 @@ size_t paged_attn_workspace_bytes(const PagedAttnArgs& a);
 // d % 8 == 0, d <= 256, 16-byte aligned rows; rows without a key become zero
 void paged_attn(const PagedAttnArgs& a, hipStream_t s);
 
-
 // Rows of queries and keys (and values, which only a cache append takes):
-// x[b][s][head][d] with strides sb / ss / sh, rows of d elements 16-byte (8-byte
-// for 16-bit types when vec == 4) aligned.
+// x[b][s][head][d] with strides sb / ss / sh, rows of d elements aligned to 16 bytes,
+// or to 8 where the type has 16 bits.
 struct RopeRows {
   const void* x = nullptr;
   const void* g = nullptr;  // backward: gradient of the output rows, strides gb / gs / gh

@@ -354,6 +354,10 @@ __host__ __device__ __forceinline__ size_t part_floats(int rows, int d) { return
 // columns each, so column = (DP / 32) * row of the tile + tile) and eight rows'
 // halves are interleaved with byte permutes.  The waves' partial (max, sum,
 // O) are joined through LDS at the end.
+// Bound by the reads of the cache: 64 single tokens after 100 to 8192, 8 heads of 128 columns, bf16: 1.10 GB in
+// 222 us, 5.0 TB/s, as a large copy; two after 131072 and 120001, fp16: 1.03 GB in 186 us, 5.5 TB/s.  One after
+// 4096: 9.5 us, the plan and a few round trips to memory.  In fp32 a block of 128 columns is 128 matrix
+// instructions of 64 cycles, about as long as a wave's share of the reads takes, and a prompt is bound by them.
 template <typename T>
 struct Elem { using type = uint16_t; static constexpr bool wide = false; };
 template <>
@@ -692,6 +696,12 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
 // lanes read 4 keys x 16 columns and each gets one column's 4 keys).  Pieces of
 // a row are stored at piece ^ turn(row), such that the 16 lanes of a read (K:
 // 16 rows, one piece; V: 4 rows, 4 pieces) touch every bank once.
+// Bound by the matrix unit and what the waves issue beside it (a block of 128 columns: a softmax of 32
+// scores a lane, 48 LDS reads, the loads' addresses): 8192 tokens, 32 heads of 128 columns, bf16, causal: 540 to 570 us, 0.96 to 1.02
+// PFLOP/s of the pairs that count, where a large matrix product reaches 1.15; 4096 tokens, 16 heads of
+// 256 columns: 190 us, 0.72; 8192 tokens, 32 heads of 64 columns: 371 us, 0.74 (as many exponentials for half
+// the products).  256 rows a workgroup share what is loaded; 128 with 256 columns, whose O fills
+// the registers of a wave.  Four pieces of V^T and six of K read ahead (two of V^T: 592 us, six: 582; four or eight of K: 578, 585).
 constexpr int kTileKeys = 64;
 
 // A row of 128 bytes shares the 256 bytes that the banks hold with its neighbour.
@@ -1034,6 +1044,8 @@ __global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile
 }
 
 // A batch of long and short pieces: the tile form's items first, the stream form's after them, one launch.
+// (700 tokens, 512 after 8488, 14 sequences of 1 and 5 tokens: 163 us with the join; the two long ones alone
+// 131 us, the others alone 42 us.  What is left is the tiles of unequal lengths, which the splits take as alike.)
 template <typename T, int DP, bool QUAD>
 __global__ __launch_bounds__(512, 2) void paged_attn_both(PagedAttnArgs t, PagedAttnArgs s, unsigned tiles) {
   if (blockIdx.x < tiles)
@@ -1048,7 +1060,8 @@ __global__ __launch_bounds__(512, 2) void paged_attn_both(PagedAttnArgs t, Paged
 // LG lanes hold a row's columns, four each; the workgroup's 256 / LG such
 // groups divide the live rows and, where there are few, a row's splits, whose
 // parts are added through LDS in a fixed order.  A pair's rows are dealt out to
-// a.apart workgroups: few pairs are spread over more of the card.
+// a.apart workgroups: few pairs are spread over more of the card.  4 to 7 us, a launch, the plan and a round
+// trip; 15 us for the tiles of that mixed batch.
 constexpr int kJoinThreads = 256;
 
 template <typename T, int ROWS, int KEYS, int LG>
