@@ -699,9 +699,8 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
 // Bound by the matrix unit and what the waves issue beside it (a block of 128 columns: a softmax of 32
 // scores a lane, 48 LDS reads, the loads' addresses): 8192 tokens, 32 heads of 128 columns, bf16, causal: 540 to 570 us, 0.96 to 1.02
 // PFLOP/s of the pairs that count, where a large matrix product reaches 1.15; 4096 tokens, 16 heads of
-// 256 columns: 190 us, 0.72; 8192 tokens, 32 heads of 64 columns: 371 us, 0.74 (as many exponentials for half
-// the products).  256 rows a workgroup share what is loaded; 128 with 256 columns, whose O fills
-// the registers of a wave.  Four pieces of V^T and six of K read ahead (two of V^T: 592 us, six: 582; four or eight of K: 578, 585).
+// 256 columns: 190 us, 0.72; 8192 tokens, 32 heads of 64 columns: 342 us, 0.80 (as many exponentials for half
+// the products).  Four pieces of V^T and six of K read ahead (two of V^T: 592 us, six: 582; four or eight of K: 578, 585).
 constexpr int kTileKeys = 64;
 
 // A row of 128 bytes shares the 256 bytes that the banks hold with its neighbour.
@@ -714,9 +713,19 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 #define NNSX_LDS __attribute__((address_space(3)))
 #define NNSX_GLOBAL __attribute__((address_space(1)))
 
-template <typename T, int DP, int WAVES, bool ONE_PAGE>
+// Waves of a workgroup.  64 columns: three workgroups of 4 waves on a compute unit (by registers) are faster
+// than one of 8 (8192 tokens, 32 heads: 342 us for 371; 4096, 16 kv heads: 75 for 93); 128 columns: one of 8 (8192 tokens,
+// 32 heads: 551 us, 579 by two of 4, which share less; 700 and 512 tokens among single ones: 164 and 206, as only
+// one fits beside the stream form's LDS); 256: one of 4, as O fills the registers of a SIMD's one wave.
+template <int DP>
+constexpr int kTileWaves = DP == 128 ? 8 : 4;
+template <int DP>
+constexpr int kTileRows = kTileWaves<DP> * kRows;
+
+template <typename T, int DP, bool ONE_PAGE>
 __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, unsigned index) {
   using E = uint16_t;
+  constexpr int WAVES = kTileWaves<DP>;
   constexpr int ROWS = WAVES * 32, NB = DP / 32, KC = DP / 16, P = DP / 8;
   constexpr int PASS = WAVES * 64 / P;       // rows of a block that the workgroup loads at once,
   constexpr int RUN = 64 / P;                // a wave's of them (1 KiB)
@@ -1038,20 +1047,20 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, unsigned index
     }
 }
 
-template <typename T, int DP, int WAVES, bool ONE_PAGE>
-__global__ __launch_bounds__(WAVES * 64, DP <= 128 ? 2 : 1) void paged_attn_tile(PagedAttnArgs a) {
-  tile_item<T, DP, WAVES, ONE_PAGE>(a, blockIdx.x);
+template <typename T, int DP, bool ONE_PAGE>
+__global__ __launch_bounds__(kTileWaves<DP> * 64, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void paged_attn_tile(PagedAttnArgs a) {
+  tile_item<T, DP, ONE_PAGE>(a, blockIdx.x);
 }
 
 // A batch of long and short pieces: the tile form's items first, the stream form's after them, one launch.
 // (700 tokens, 512 after 8488, 14 sequences of 1 and 5 tokens: 163 us with the join; the two long ones alone
 // 131 us, the others alone 42 us.  What is left is the tiles of unequal lengths, which the splits take as alike.)
 template <typename T, int DP, bool QUAD>
-__global__ __launch_bounds__(512, 2) void paged_attn_both(PagedAttnArgs t, PagedAttnArgs s, unsigned tiles) {
+__global__ __launch_bounds__(kTileWaves<DP> * 64, DP <= 64 ? 3 : 2) void paged_attn_both(PagedAttnArgs t, PagedAttnArgs s, unsigned tiles) {
   if (blockIdx.x < tiles)
-    tile_item<T, DP, 8, false>(t, blockIdx.x);
+    tile_item<T, DP, false>(t, blockIdx.x);
   else
-    stream_item<T, DP, QUAD, 8>(s, blockIdx.x - tiles);
+    stream_item<T, DP, QUAD, kTileWaves<DP>>(s, blockIdx.x - tiles);
 }
 
 // ------------------------------------------------------------------- join ----
@@ -1174,23 +1183,13 @@ void launch_stream(const PagedAttnArgs& a, unsigned grid, hipStream_t s) {
     paged_attn_stream<T, DP, false><<<grid, kThreads, 0, s>>>(a);
 }
 
-template <typename T>
-void launch_stream(const PagedAttnArgs& a, hipStream_t s) {
-  const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(a.slots) * a.hkv);
-  if (a.d <= 64)
-    launch_stream<T, 64>(a, grid, s);
-  else if (a.d <= 128)
-    launch_stream<T, 128>(a, grid, s);
-  else
-    launch_stream<T, 256>(a, grid, s);
-}
-
-template <typename T, int DP, int WAVES>
+template <typename T, int DP>
 void launch_tile(const PagedAttnArgs& a, unsigned grid, hipStream_t s) {
+  constexpr int threads = kTileWaves<DP> * 64;
   if (DP > 128 && a.p.page % (512 / DP) == 0)  // (the keys of 1 KiB)
-    paged_attn_tile<T, DP, WAVES, (DP > 128)><<<grid, WAVES * 64, 0, s>>>(a);
+    paged_attn_tile<T, DP, (DP > 128)><<<grid, threads, 0, s>>>(a);
   else
-    paged_attn_tile<T, DP, WAVES, false><<<grid, WAVES * 64, 0, s>>>(a);
+    paged_attn_tile<T, DP, false><<<grid, threads, 0, s>>>(a);
 }
 
 // (sequence, tile) pairs a call can have: every sequence, and the rows behind the last, may end in a partial tile
@@ -1198,7 +1197,7 @@ int64_t pairs_bound(const PagedAttnArgs& a, int rows) {
   return static_cast<int64_t>(a.p.T) * a.group / rows + std::min<int64_t>(a.p.B + 1, a.p.T);
 }
 
-int tile_rows(const PagedAttnArgs& a) { return a.d <= 128 ? 256 : 128; }
+int tile_rows(const PagedAttnArgs& a) { return a.d <= 64 ? kTileRows<64> : a.d <= 128 ? kTileRows<128> : kTileRows<256>; }
 
 // Either form's part of a call: which sequences it takes (by their rows), and
 // how its keys are split: for about `target` items a kv head (0: no split), of at least `min_chunk` key blocks.
@@ -1221,6 +1220,9 @@ PagedAttnArgs part_of(const PagedAttnArgs& a0, int rows, int64_t pairs, int rows
 size_t part_bytes(const PagedAttnArgs& a, int rows) {
   return static_cast<size_t>(2 * a.target) * a.hkv * part_floats(rows, a.d) * sizeof(float);
 }
+
+// workgroups of the tile form, or of both, that a compute unit holds
+int tile_units(const PagedAttnArgs& a) { return a.d <= 64 ? 3 : 1; }
 
 constexpr int kAllRows = 0x7fffffff;
 // Rows of a sequence up to which the stream form takes it: one item's.  (30 x 16 tokens, 64 rows, beside 2 x 1024,
@@ -1253,19 +1255,23 @@ Plan plan_of(PagedAttnArgs a) {
   // 8 items a compute unit, where its workgroups are alone (60 single tokens after 8192: 362 us, from 2 a unit on 516 us, as
   // 480 items are nearly a round already), of which the rounds decide (8 tokens after 4096: 35 us, always 8 a unit 48 us;
   // 1 after 131072: 105 us and 125 us; 24 after 2048 to 16384, 4 heads: 102 us and 112 us).
-  const int per_cu = p.tile ? 2 : a.type == AttnType::kF32 ? 3 : 8;
+  const int per_cu = p.tile ? 2 * tile_units(a) : a.type == AttnType::kF32 ? 3 : 8;
   const int64_t pairs = p.tile ? static_cast<int64_t>(a.p.B) + 1 : pairs_bound(a, kRows);  // (with the tile form: one a sequence)
   p.s = part_of(a, kRows, pairs, 0, p.tile ? kStreamRows : kAllRows, per_cu * kCus, p.tile ? 8 : 4);
-  p.s.one_round = ((p.tile || (a.type == AttnType::kF32 && a.d > 64) ? 1 : 2) * kCus + a.hkv - 1) / a.hkv;
+  const int units = p.tile ? tile_units(a) : a.type == AttnType::kF32 && a.d > 64 ? 1 : 2;
+  p.s.one_round = (units * kCus + a.hkv - 1) / a.hkv;
   p.s.item_cost = a.type == AttnType::kF32 ? 6 : 16;
   // The tile form splits where whole tiles do not fill the card (1300 tokens after 8192, 168 tiles: 212 us,
   // 317 us whole; 3600 tokens after 16384, 456 tiles: 852 us, 1065 us if those split too: a
   // split's rows go through memory twice).  Splits of less than 8 blocks cost more than they give
   // (4 x 100 tokens alone: 25.7 us, 29.1 us with splits of 4).
+  // 64 columns and less: three times as many tiles fill it, but from twice as many on whole ones are faster
+  // (4096 tokens, 16 heads: 75 us, 90 us split; 1500 tokens after 16384: 281 us, 330 us whole).
   const int64_t tiles = (rows + tile_rows(a) - 1) / tile_rows(a) * a.hkv;
+  const int slots = tile_units(a) * kCus, full = std::min(slots, 2 * kCus);
   p.t = part_of(a, tile_rows(a), pairs_bound(a, tile_rows(a)), p.stream ? kStreamRows : 0, kAllRows,
-                tiles >= kCus ? 0 : 2 * kCus, 8);
-  p.t.one_round = (kCus + a.hkv - 1) / a.hkv;
+                tiles >= full ? 0 : 2 * slots, 8);
+  p.t.one_round = (slots + a.hkv - 1) / a.hkv;
   p.t.item_cost = 8;
   p.t.ws = static_cast<char*>(a.ws) + (p.stream ? part_bytes(p.s, kRows) : 0);
   return p;
@@ -1273,48 +1279,48 @@ Plan plan_of(PagedAttnArgs a) {
 
 unsigned grid_of(const PagedAttnArgs& a) { return static_cast<unsigned>(static_cast<int64_t>(a.slots) * a.hkv); }
 
-template <typename T, int TILE_ROWS>
+template <typename T, int DP>
 void launch_join(const Plan& p, hipStream_t s) {
   const auto wgs = [](bool runs, const PagedAttnArgs& a) {
     return runs && a.target > 0 ? static_cast<unsigned>(static_cast<int64_t>(a.pairs) * a.hkv * a.apart) : 0u;
   };
   const unsigned tiles = wgs(p.tile, p.t), grid = tiles + wgs(p.stream, p.s);
-  if (grid == 0) return;
-  if (p.s.d <= 64)
-    paged_attn_join<T, TILE_ROWS, 16><<<grid, kJoinThreads, 0, s>>>(p.t, p.s, tiles);
-  else if (p.s.d <= 128)
-    paged_attn_join<T, TILE_ROWS, 32><<<grid, kJoinThreads, 0, s>>>(p.t, p.s, tiles);
-  else
-    paged_attn_join<T, TILE_ROWS, 64><<<grid, kJoinThreads, 0, s>>>(p.t, p.s, tiles);
+  if (grid > 0) paged_attn_join<T, Elem<T>::wide ? 0 : kTileRows<DP>, DP / 4><<<grid, kJoinThreads, 0, s>>>(p.t, p.s, tiles);
 }
 
 template <typename T, int DP>
 void launch_both(const Plan& p, hipStream_t s) {
   const unsigned tiles = grid_of(p.t), grid = tiles + grid_of(p.s);
+  constexpr int threads = kTileWaves<DP> * 64;
   if (p.t.p.page % 4 == 0)
-    paged_attn_both<T, DP, true><<<grid, 512, 0, s>>>(p.t, p.s, tiles);
+    paged_attn_both<T, DP, true><<<grid, threads, 0, s>>>(p.t, p.s, tiles);
   else
-    paged_attn_both<T, DP, false><<<grid, 512, 0, s>>>(p.t, p.s, tiles);
+    paged_attn_both<T, DP, false><<<grid, threads, 0, s>>>(p.t, p.s, tiles);
+}
+
+template <typename T, int DP>
+void launch(const Plan& p, hipStream_t s) {
+  if constexpr (!Elem<T>::wide) {
+    if constexpr (DP <= 128) {
+      if (p.tile && p.stream) {
+        launch_both<T, DP>(p, s);
+        return launch_join<T, DP>(p, s);
+      }
+    }  // (else the two forms' LDS does not fit one workgroup)
+    if (p.tile) launch_tile<T, DP>(p.t, grid_of(p.t), s);
+  }
+  if (p.stream) launch_stream<T, DP>(p.s, grid_of(p.s), s);
+  launch_join<T, DP>(p, s);
 }
 
 template <typename T>
 void launch(const Plan& p, hipStream_t s) {
-  if constexpr (!Elem<T>::wide) {
-    if (p.tile) {
-      if (p.s.d > 128) {  // (the two forms' LDS does not fit one workgroup)
-        launch_tile<T, 256, 4>(p.t, grid_of(p.t), s);
-        if (p.stream) launch_stream<T>(p.s, s);
-        return launch_join<T, 128>(p, s);
-      }
-      if (p.s.d <= 64)
-        p.stream ? launch_both<T, 64>(p, s) : launch_tile<T, 64, 8>(p.t, grid_of(p.t), s);
-      else
-        p.stream ? launch_both<T, 128>(p, s) : launch_tile<T, 128, 8>(p.t, grid_of(p.t), s);
-      return launch_join<T, 256>(p, s);
-    }
-  }
-  launch_stream<T>(p.s, s);
-  launch_join<T, 0>(p, s);
+  if (p.s.d <= 64)
+    launch<T, 64>(p, s);
+  else if (p.s.d <= 128)
+    launch<T, 128>(p, s);
+  else
+    launch<T, 256>(p, s);
 }
 
 }  // namespace
