@@ -261,8 +261,8 @@ __device__ __forceinline__ int64_t position_of(const RopeArgs& a, int b, int s) 
 
 // --------------------------------------------------------------- forward ----
 // blockIdx.x: token, blockIdx.y: slice of the heads (q, then k, then v).
-// Bound by its bytes: 8192 tokens, 40 heads of 128 columns, bf16: 172 MB in 31 us, 5.5 TB/s
-// (a large copy: 5.0); as an append of 8192 fp16 tokens, 48 heads: 206 MB in 38 us, 5.4 TB/s.
+// Bound by its bytes: 8192 tokens, 40 heads of 128 columns, bf16: 172 MB in 38 us, 4.6 TB/s
+// (a large copy: 5.0; 28 us where the caches hold the rows); as an append of 8192 fp16 tokens, 48 heads: 206 MB in 48 us, 4.3 TB/s.
 // 8 tokens: 5 us, the launch and one round trip to memory.
 template <typename T, int VEC, int LPR, bool INTER, bool APPEND>
 __global__ __launch_bounds__(512) void rope_forward(RopeArgs a) {
@@ -275,6 +275,20 @@ __global__ __launch_bounds__(512) void rope_forward(RopeArgs a) {
   const int h = is_q ? head : is_v ? head - a.q.heads - a.k.heads : head - a.q.heads;
   const RopeRows& r = is_q ? a.q : is_v ? a.v : a.k;
   const Lane<VEC> l = lane_of<VEC, INTER>(j, a.d, a.rot);
+
+  const E* xp = static_cast<const E*>(r.x) + b * r.sb + s * r.ss + h * r.sh;
+  Raw<T, VEC> xr[2]{};
+  float w[2 * VEC];
+  if constexpr (APPEND) {
+    // the row and its weight are under way while the position is found, three loads one after the other
+    // (8192 tokens of five sequences: 48 us, 55 us with the row after them)
+    if (head < heads) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (l.has[e]) xr[e].load(xp + l.c[e]);
+      if (a.norm && !is_v) load_weight<T, VEC>(r.w, a.w_f32, l, w);
+    }
+  }
 
   // where the token stands, and the cache row its key and value go to
   int64_t pos;
@@ -308,22 +322,26 @@ __global__ __launch_bounds__(512) void rope_forward(RopeArgs a) {
   }
   if (head >= heads) return;
 
-  const E* xp = static_cast<const E*>(r.x) + b * r.sb + s * r.ss + h * r.sh;
   float x[2 * VEC];
-  Raw<T, VEC> xr[2]{};
-  if (pos >= 0) {
+  if constexpr (!APPEND) {
+    if (pos >= 0) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
-      if (l.has[e]) xr[e].load(xp + l.c[e]);
+      for (int e = 0; e < 2; ++e)
+        if (l.has[e]) xr[e].load(xp + l.c[e]);
+    }
   }
-  float cs[VEC], sn[VEC], w[2 * VEC];
+  float cs[VEC], sn[VEC];
   const bool turns = !is_v && pos >= 0;
   if (turns) {  // (every load before the first use)
     load_angles<VEC, INTER>(a.rope == nullptr ? nullptr : a.rope + pos * a.rstride, l, a.rot, cs, sn);
-    if (a.norm) load_weight<T, VEC>(r.w, a.w_f32, l, w);
+    if (!APPEND && a.norm) load_weight<T, VEC>(r.w, a.w_f32, l, w);
   }
 #pragma unroll
   for (int e = 0; e < 2; ++e) xr[e].unpack(x + e * VEC);
+  if (APPEND && pos < 0) {  // (whatever the row holds)
+#pragma unroll
+    for (int i = 0; i < 2 * VEC; ++i) x[i] = 0.f;
+  }
   if (turns) {
     if (a.norm) {
       float ss = 0.f;
@@ -352,9 +370,9 @@ __global__ __launch_bounds__(512) void rope_forward(RopeArgs a) {
 // weight gradient of its own columns in registers; at the end the workgroup's
 // rows are added in LDS in a fixed order and its partial sums stored, and a second kernel
 // adds the workgroups' -- no atomics, the same result every time.
-// 8192 tokens, 40 heads of 128 columns, bf16: 256 MB in 69 us, 3.7 TB/s (51 us where the caches still hold
-// the rows), and 4 us for the sum: bound by how many loads 10 waves a compute unit keep under way
-// (more waves and their partial sums are slower in all, see backward_blocks).
+// 8192 tokens, 40 heads of 128 columns, bf16: 256 MB in 67 us with the sum of 4, 4.1 TB/s (51 us where the caches
+// hold the rows).  More waves, more rows loaded ahead and consecutive tokens for a workgroup were all slower
+// (87, 70 and 71 us).
 template <typename T, int VEC, int LPR, bool INTER>
 __global__ __launch_bounds__(512, 4) void rope_backward(RopeArgs a) {
   using E = typename T::E;
@@ -570,7 +588,7 @@ void forward(const RopeArgs& a, hipStream_t s) {
 }
 
 // Workgroups along the tokens of the backward kernel: about ten waves a compute unit in all, one round
-// (8192 tokens x 40 heads x 128 bf16: 512 workgroups of 5 waves 51 us with the sum, 768 62 us, 1024 66 us)
+// (8192 tokens x 40 heads x 128 bf16: 512 workgroups of 5 waves 67 us with the sum, 256 97 us, 768 82 us, 1024 86 us)
 int backward_blocks(const RopeArgs& a, int threads, int slices) {
   const int waves = threads / 64 * slices;
   return static_cast<int>(std::min<int64_t>(static_cast<int64_t>(a.B) * a.S, std::max(2560 / waves, 1)));
