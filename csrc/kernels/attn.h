@@ -41,7 +41,7 @@ struct PagedAttnArgs {
   int window = 0;       // 0: no window; else keys in (position - window, position]
   void* ws = nullptr;   // paged_attn_workspace_bytes(a)
   // derived by the launcher: rows a token, and how the keys are split (attn.hip, plan)
-  int group = 1, target = 0, min_chunk = 1, slots = 0, pairs = 0, apart = 1, one_round = 0, item_cost = 0, rows_lo = 0, rows_hi = 0;
+  int group = 1, target = 0, min_chunk = 1, slots = 0, pairs = 0, parts = 0, apart = 1, one_round = 0, item_cost = 0, rows_lo = 0, rows_hi = 0;
 };
 // bytes of scratch memory the call needs (0: none)
 size_t paged_attn_workspace_bytes(const PagedAttnArgs& a);

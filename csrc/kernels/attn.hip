@@ -305,7 +305,7 @@ __device__ Item find_item(const PagedAttnArgs& a, int index) {
       it.len = get(s.len);
       it.keys = get(s.keys);
       // (offsets that do not ascend may make more items than planned for: those are left out)
-      if (it.splits == 1 || (it.part >= 0 && it.part <= 2 * a.target - (PAIRS ? it.splits : 1))) it.b = b0 + l;
+      if (it.splits == 1 || (it.part >= 0 && it.part <= a.parts - (PAIRS ? it.splits : 1))) it.b = b0 + l;
       return it;
     }
     before.pairs += last_lane(pairs);
@@ -1212,13 +1212,14 @@ PagedAttnArgs part_of(const PagedAttnArgs& a0, int rows, int64_t pairs, int rows
   a.min_chunk = min_chunk;
   a.pairs = static_cast<int>(pairs);
   a.slots = static_cast<int>(std::min<int64_t>(pairs + a.target, pairs * most));
+  a.parts = std::min(2 * a.target, a.slots);  // (items of split pairs)
   a.apart = static_cast<int>(std::clamp<int64_t>(rows / kRows * 4 * kCus / (static_cast<int64_t>(a.pairs) * a.hkv), 1,
                                                  rows > kRows ? rows / 32 : kRows));
   return a;
 }
 
 size_t part_bytes(const PagedAttnArgs& a, int rows) {
-  return static_cast<size_t>(2 * a.target) * a.hkv * part_floats(rows, a.d) * sizeof(float);
+  return static_cast<size_t>(a.parts) * a.hkv * part_floats(rows, a.d) * sizeof(float);
 }
 
 // workgroups of the tile form, or of both, that a compute unit holds
