@@ -225,6 +225,37 @@ def test_refusals_of_append(ops):
     refused("no gradient", call, rope=rope.clone().requires_grad_(True))
 
 
+def test_qk_norm_rope_part_of_the_gradient(ops):
+    """one output used, inputs that ask for none, the graph used twice and given back"""
+    torch.manual_seed(3)
+    q, k, w = torch.randn(5, 4, 16), torch.randn(5, 2, 16), torch.rand(16) + 0.5
+    pos, rope = torch.arange(5), ops.rope_table(5, 16)
+    g = torch.randn(5, 2, 16)
+    full = ops.qk_norm_rope_backward(torch.zeros_like(q), g, q, k, w, w, pos, rope)
+    a = [x.clone().requires_grad_(True) for x in (q, k, w, w)]
+    _, yk = ops.qk_norm_rope(*a, pos, rope)
+    got = torch.autograd.grad(yk, a, g, retain_graph=True)
+    assert all(torch.equal(x, y) for x, y in zip(got, full)) and (got[0] == 0).all()
+    assert torch.equal(torch.autograd.grad(yk, a[1], g)[0], full[1])
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(yk, a[1], g)
+    k2 = k.clone().requires_grad_(True)
+    yq, yk = ops.qk_norm_rope(q, k2, None, w, pos, rope)
+    assert yq.requires_grad and yk.requires_grad
+    yk.backward(g)
+    assert torch.equal(k2.grad, full[1]) and q.grad is None
+    k2 = k.clone().requires_grad_(True)
+    _, yk = ops.qk_norm_rope(q, k2 * 1.0, None, None, pos, rope)
+    assert not ops.qk_norm_rope(q, k, w, w, pos, rope)[0].requires_grad
+    with torch.no_grad():
+        assert not ops.qk_norm_rope(q, k2, w, w, pos, rope)[1].requires_grad
+    x = k.clone().requires_grad_(True) * 1.0
+    _, yk = ops.qk_norm_rope(q, x, None, None, pos, rope)
+    x.add_(1.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        yk.sum().backward()
+
+
 def test_append_is_seen_by_gradients(ops):
     """a cache that an earlier operation keeps for its gradient is not changed unnoticed"""
     s = ref.batch([2, 1], [5, 9], 4, 2, 16, 4, torch.float32)
