@@ -144,7 +144,8 @@ __device__ __forceinline__ float row_sum(float x) {
 
 // ------------------------------------------------------------------- plan ----
 // Work is cut into items: (sequence, tile of rows, split of its key blocks).
-// Lengths live on the device, so every wave derives its own item from them: the
+// Lengths live on the device, so every wave derives its own item from them (of many
+// sequences, from what one workgroup has summed up before): the
 // key blocks of all (sequence, tile) pairs are summed, a split is chosen so long
 // that about `target` items result (more only because every pair has at least
 // one), and the item's pair is found by a running sum over the sequences.
@@ -237,14 +238,65 @@ __device__ __forceinline__ int splits_of(const Seq& s, int chunk) {
   return s.blocks > chunk ? static_cast<int>(static_cast<uint32_t>(s.blocks + chunk - 1) / static_cast<uint32_t>(chunk)) : 1;
 }
 
+// Many sequences: what stands before each, [B + 1], and behind them the key blocks of a split, all
+// written by one workgroup in a launch before the others.  (Single tokens after 512, us with and without: 256 sequences 117 and
+// 136, 1024 402 and 655; 128 after 1024 128 and 127, with two prompts of 512 among them 187 and 204.)
+struct PlanEntry {
+  int pairs;
+  uint32_t split;  // as in Count
+};
+
+// item number `rel` of a sequence, `first_split` before it
+template <bool PAIRS>
+__device__ __forceinline__ Item item_of(const PagedAttnArgs& a, int b, const Seq& s, int rel, int splits, int chunk, uint32_t first_split) {
+  Item it;
+  it.splits = splits;
+  const int tile = PAIRS ? rel : rel / splits;
+  it.split = PAIRS ? 0 : rel - tile * splits;
+  it.tile = s.tiles - 1 - tile;  // the tiles with the most keys first: the short ones fill the tail
+  it.part = static_cast<int>(first_split & 0xffff) + tile * splits + it.split;
+  it.chunk = chunk;
+  it.n = s.n;
+  it.t0 = s.t0;
+  it.len = s.len;
+  it.keys = s.keys;
+  // (offsets that do not ascend may make more items than planned for: those are left out)
+  it.b = splits == 1 || (it.part >= 0 && it.part <= a.parts - (PAIRS ? splits : 1)) ? b : -1;
+  return it;
+}
+
+template <int ROWS, int KEYS, bool PAIRS>
+__device__ __forceinline__ Item find_planned(const PagedAttnArgs& a, int index) {
+  const PlanEntry* plan = static_cast<const PlanEntry*>(a.plan);
+  const int lane = threadIdx.x & 63, B1 = a.p.B + 1;
+  auto first_of = [&](const PlanEntry& e) { return PAIRS ? e.pairs : e.pairs + static_cast<int>(e.split >> 16); };
+  // the last sequence that begins at or before the item, by 64 steps at a time
+  int lo = 0;
+  for (int n = B1, step = 0; step != 1; n = min(step, B1 - lo)) {
+    step = (n + 63) / 64;
+    const int i = lane * step;
+    const int c = __popcll(__ballot(i < n && first_of(plan[lo + min(i, n - 1)]) <= index));
+    lo += max(c - 1, 0) * step;
+  }
+  const PlanEntry e = plan[lo];
+  const int chunk = plan[B1].pairs;
+  const Seq s = seq_of<ROWS, KEYS>(a, lo);
+  const int splits = splits_of(s, chunk), rel = index - first_of(e);
+  if (rel < 0 || rel >= s.tiles * (PAIRS ? 1 : splits)) {
+    Item none;
+    none.b = -1;
+    return none;
+  }
+  return item_of<PAIRS>(a, lo, s, rel, splits, chunk, e.split);
+}
+
 // PAIRS false: `index` counts items; PAIRS true: (sequence, tile) pairs, and
 // the item is the pair's first split.  Each wave finds it by itself among 64
 // sequences at a time; more are summed up first, 64 at a time, by every wave.
 template <int ROWS, int KEYS, bool PAIRS>
 __device__ Item find_item(const PagedAttnArgs& a, int index) {
 #pragma clang fp contract(off)  // (the kernels of a call have to agree on the plan)
-  Item it;
-  it.b = -1;
+  if (a.plan != nullptr) return find_planned<ROWS, KEYS, PAIRS>(a, index);
   const int lane = threadIdx.x & 63, B1 = a.p.B + 1;
   Seq s{};
   if (lane < B1) s = seq_of<ROWS, KEYS>(a, lane);
@@ -293,25 +345,61 @@ __device__ Item find_item(const PagedAttnArgs& a, int index) {
     if (here != 0) {
       const int l = __builtin_ctzll(here);
       auto get = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
-      const int rel = index - get(first);
-      it.splits = get(splits);
-      const int tile = PAIRS ? rel : rel / it.splits;
-      it.split = PAIRS ? 0 : rel - tile * it.splits;
-      it.tile = get(s.tiles) - 1 - tile;  // the tiles with the most keys first: the short ones fill the tail
-      it.part = (get(static_cast<int>(first_split)) & 0xffff) + tile * it.splits + it.split;
-      it.chunk = chunk;
-      it.n = get(s.n);
-      it.t0 = get(s.t0);
-      it.len = get(s.len);
-      it.keys = get(s.keys);
-      // (offsets that do not ascend may make more items than planned for: those are left out)
-      if (it.splits == 1 || (it.part >= 0 && it.part <= a.parts - (PAIRS ? it.splits : 1))) it.b = b0 + l;
-      return it;
+      const Seq found{get(s.n), get(s.t0), get(s.len), get(s.keys), get(s.tiles), get(s.blocks)};
+      return item_of<PAIRS>(a, b0 + l, found, index - get(first), get(splits), chunk, static_cast<uint32_t>(get(static_cast<int>(first_split))));
     }
     before.pairs += last_lane(pairs);
     before.split += static_cast<uint32_t>(last_lane(static_cast<int>(split)));
   }
-  return it;
+  Item none;
+  none.b = -1;
+  return none;
+}
+
+constexpr int kPlanThreads = 1024;
+
+template <int ROWS, int KEYS>
+__device__ void make_plan(const PagedAttnArgs& a) {
+#pragma clang fp contract(off)
+  __shared__ float sums[kPlanThreads / 64];
+  __shared__ Count ends[kPlanThreads / 64];
+  PlanEntry* plan = static_cast<PlanEntry*>(a.plan);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, B1 = a.p.B + 1;
+  float work = 0.f;
+  if (a.target > 0)
+    for (int b = threadIdx.x; b < B1; b += kPlanThreads) {
+      const Seq s = seq_of<ROWS, KEYS>(a, b);
+      work += static_cast<float>(s.tiles) * static_cast<float>(s.blocks);
+    }
+  work = wave_scan(work);
+  if (lane == 63) sums[wave] = work;
+  __syncthreads();
+  work = 0.f;
+  for (int w = 0; w < kPlanThreads / 64; ++w) work += sums[w];
+  const int chunk = chunk_of(a, work);
+  Count before{0, 0};
+  for (int b0 = 0; b0 < B1; b0 += kPlanThreads) {
+    const int b = b0 + static_cast<int>(threadIdx.x);
+    Seq s{};
+    if (b < B1) s = seq_of<ROWS, KEYS>(a, b);
+    const Count mine = count_of(s, splits_of(s, chunk));
+    const int pairs = wave_scan(mine.pairs);
+    const uint32_t split = static_cast<uint32_t>(wave_scan(static_cast<int>(mine.split)));
+    if (lane == 63) ends[wave] = {pairs, split};
+    __syncthreads();
+    Count here = before;
+    for (int w = 0; w < kPlanThreads / 64; ++w) {
+      if (w < wave) {
+        here.pairs += ends[w].pairs;
+        here.split += ends[w].split;
+      }
+      before.pairs += ends[w].pairs;
+      before.split += ends[w].split;
+    }
+    if (b < B1) plan[b] = {here.pairs + pairs - mine.pairs, here.split + split - mine.split};
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) plan[B1] = {chunk, 0u};
 }
 
 // keys [lo, hi) that the tokens i0 .. i1 of an item see
@@ -1165,6 +1253,15 @@ __device__ __forceinline__ void join_pair(const PagedAttnArgs& a, unsigned index
   }
 }
 
+template <int TILE_ROWS>
+__global__ __launch_bounds__(kPlanThreads) void paged_attn_plan(PagedAttnArgs t, PagedAttnArgs s) {
+  if (blockIdx.x == 0) {
+    if (s.plan != nullptr) make_plan<kRows, kKeys>(s);
+  } else {
+    if (t.plan != nullptr) make_plan<TILE_ROWS, kTileKeys>(t);
+  }
+}
+
 // `tiles` workgroups for the tile form's pairs, then the stream form's
 template <typename T, int TILE_ROWS, int LG>
 __global__ __launch_bounds__(kJoinThreads) void paged_attn_join(PagedAttnArgs t, PagedAttnArgs s, unsigned tiles) {
@@ -1225,6 +1322,10 @@ size_t part_bytes(const PagedAttnArgs& a, int rows) {
 // workgroups of the tile form, or of both, that a compute unit holds
 int tile_units(const PagedAttnArgs& a) { return a.d <= 64 ? 3 : 1; }
 
+// Sequences from which on a plan is made
+constexpr int kPlanned = 128;
+size_t plan_bytes(const PagedAttnArgs& a) { return (static_cast<size_t>(a.p.B) + 2) * sizeof(PlanEntry); }
+
 constexpr int kAllRows = 0x7fffffff;
 // Rows of a sequence up to which the stream form takes it: one item's.  (30 x 16 tokens, 64 rows, beside 2 x 1024,
 // all after 4096: 289 us; 397 us if the stream form takes them, which then reads each key twice.)
@@ -1274,7 +1375,14 @@ Plan plan_of(PagedAttnArgs a) {
                 tiles >= full ? 0 : 2 * slots, 8);
   p.t.one_round = (slots + a.hkv - 1) / a.hkv;
   p.t.item_cost = 8;
-  p.t.ws = static_cast<char*>(a.ws) + (p.stream ? part_bytes(p.s, kRows) : 0);
+  char* ws = static_cast<char*>(a.ws) + (p.stream ? part_bytes(p.s, kRows) : 0);
+  p.t.ws = ws;
+  ws += p.tile ? part_bytes(p.t, tile_rows(a)) : 0;
+  p.s.plan = p.t.plan = nullptr;
+  if (a.p.B >= kPlanned) {
+    if (p.stream) p.s.plan = ws;
+    if (p.tile) p.t.plan = ws + plan_bytes(a);
+  }
   return p;
 }
 
@@ -1301,6 +1409,8 @@ void launch_both(const Plan& p, hipStream_t s) {
 
 template <typename T, int DP>
 void launch(const Plan& p, hipStream_t s) {
+  if (p.s.p.B >= kPlanned)
+    paged_attn_plan<Elem<T>::wide ? kRows : kTileRows<DP>><<<p.tile ? 2 : 1, kPlanThreads, 0, s>>>(p.t, p.s);
   if constexpr (!Elem<T>::wide) {
     if constexpr (DP <= 128) {
       if (p.tile && p.stream) {
@@ -1328,7 +1438,8 @@ void launch(const Plan& p, hipStream_t s) {
 
 size_t paged_attn_workspace_bytes(const PagedAttnArgs& a) {
   const Plan p = plan_of(a);
-  return (p.stream ? part_bytes(p.s, kRows) : 0) + (p.tile ? part_bytes(p.t, tile_rows(a)) : 0);
+  return (p.stream ? part_bytes(p.s, kRows) : 0) + (p.tile ? part_bytes(p.t, tile_rows(a)) : 0) +
+         (a.p.B >= kPlanned ? 2 * plan_bytes(a) : 0);
 }
 
 void paged_attn(const PagedAttnArgs& a, hipStream_t s) {

@@ -294,12 +294,14 @@ __global__ __launch_bounds__(512) void rope_forward(RopeArgs a) {
   int64_t pos;
   int64_t krow = -1, vrow = -1;
   if constexpr (APPEND) {
-    // sequence: how many of cu[1 .. B] lie at or before the token (a wave counts 64 at once)
+    // sequence: the last that starts at or before the token, by 64 steps at a time
     const int lane = threadIdx.x & 63;
     int seq = 0;
-    for (int i0 = 1; i0 <= a.p.B; i0 += 64) {
-      const int n = __popcll(__ballot(i0 + lane <= a.p.B && a.p.cu[min(i0 + lane, a.p.B)] <= s));
-      seq += n;
+    for (int n = a.p.B + 1, step = 0; step != 1; n = min(step, a.p.B + 1 - seq)) {
+      step = (n + 63) / 64;
+      const int i = lane * step, at = seq + min(i, n - 1);
+      const int c = __popcll(__ballot(i < n && (at == 0 || a.p.cu[at] <= s)));
+      seq += max(c - 1, 0) * step;
     }
     pos = -1;
     if (seq < a.p.B) {

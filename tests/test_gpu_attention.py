@@ -90,6 +90,36 @@ def test_paged_attention_many_splits(ops, lens, new):
     check(ops, ref.batch([new] * len(kv), kv, 8, 2, 64, 16, torch.bfloat16, "cuda", pad=2))
 
 
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 64), (torch.float16, 128), (torch.bfloat16, 256), (torch.float32, 64)])
+@pytest.mark.parametrize("count", [127, 128, 1100])
+def test_paged_attention_hundreds_of_sequences(ops, dtype, dim, count):
+    """single tokens, empty sequences, chunks and one long sequence among hundreds; rows behind the last"""
+    new = [(1, 1, 0, 1, 3)[i % 5] for i in range(count)]
+    kv = [n + (i * 37) % 70 for i, n in enumerate(new)]
+    new[count // 2], kv[count // 2] = 60, 90
+    kv[7] = 4000
+    s = ref.batch(new, kv, 4, 2, dim, 16, dtype, "cuda", pad=40)
+    check(ops, s)
+    got = check(ops, s, window=33)
+    assert (got[sum(new):] == 0).all()
+    assert torch.equal(attend(ops, s, window=33), got)
+    s = ref.batch([1] * count, [(i * 29) % 90 for i in range(count)], 4, 2, dim, 16, dtype, "cuda")
+    check(ops, s)
+
+
+def test_paged_attention_of_a_million_rows(ops):
+    """2^20 tokens that see themselves only: the output is their value"""
+    t, page = 1 << 20, 64
+    pages = t // page + 2
+    kc, vc = (torch.randn(pages, 1, page, 8, device="cuda").bfloat16() for _ in range(2))
+    table = torch.randperm(pages, device="cuda").int()[None]
+    q = torch.randn(t, 2, 8, device="cuda").bfloat16()
+    got = ops.paged_attention(q, kc, vc, table, ints(0, t - 3), ints(t + 50), window=1)
+    key = torch.arange(t - 3, device="cuda") + 53
+    want = vc[table[0, key // page].long(), 0, key % page]
+    assert torch.equal(got[:t - 3], want[:, None].expand(-1, 2, -1)) and (got[t - 3:] == 0).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_paged_attention_empty_slots(ops, dtype):
     """a batch of fixed slots, most of them empty: prompts among them, as many tokens as slots"""
