@@ -239,8 +239,9 @@ __device__ __forceinline__ int splits_of(const Seq& s, int chunk) {
 }
 
 // Many sequences: what stands before each, [B + 1], and behind them the key blocks of a split, all
-// written by one workgroup in a launch before the others.  (Single tokens after 512, us with and without: 256 sequences 117 and
-// 136, 1024 402 and 655; 128 after 1024 128 and 127, with two prompts of 512 among them 187 and 204.)
+// written by one workgroup in a launch before the others.  (Where every wave looked through all sequences instead,
+// 64 at a time: 1024 single tokens after 512 655 us, 408 by the plan; 256 136 and 119; 64 after 1024, which
+// were not weighed then, 70 and 54.)
 struct PlanEntry {
   int pairs;
   uint32_t split;  // as in Count
@@ -290,70 +291,63 @@ __device__ __forceinline__ Item find_planned(const PagedAttnArgs& a, int index) 
   return item_of<PAIRS>(a, lo, s, rel, splits, chunk, e.split);
 }
 
+// The card takes `one_round` items of a kv head at once: items just beyond a round take a whole
+// one more, and each has a cost of its own.  So of the splits 1, 1 1/8, .. 8 7/8 times as long
+// as the shortest, one a lane, the one with the least rounds times blocks is taken (by estimate:
+// products with reciprocals).
+__device__ __forceinline__ int longer(int chunk, int lane) { return chunk + chunk / 8 * lane + chunk % 8 * lane / 8; }
+__device__ __forceinline__ float items_by(int tiles, int blocks, float of_chunk) {
+  return static_cast<float>(tiles) * fmaxf(ceilf(static_cast<float>(blocks) * of_chunk - 1e-3f), 1.f);
+}
+// this lane's items of the wave's sequences
+__device__ __forceinline__ float weigh_wave(const Seq& s, int chunk) {
+  const float of = __builtin_amdgcn_rcpf(static_cast<float>(chunk));
+  float items = 0.f;
+  for (uint64_t left = __ballot(s.tiles > 0); left != 0; left &= left - 1) {
+    const int l = __builtin_ctzll(left);
+    items += items_by(__builtin_amdgcn_readlane(s.tiles, l), __builtin_amdgcn_readlane(s.blocks, l), of);
+  }
+  return items;
+}
+__device__ __forceinline__ int best_of(const PagedAttnArgs& a, int chunk, float items) {
+  const float round = __builtin_amdgcn_rcpf(static_cast<float>(a.one_round));
+  const float cost = ceilf(items * round - 1e-3f) * static_cast<float>(chunk + a.item_cost);
+  return __builtin_amdgcn_readlane(chunk, __builtin_ctzll(__ballot(cost == last_lane(wave_least(cost)))));
+}
+
 // PAIRS false: `index` counts items; PAIRS true: (sequence, tile) pairs, and
-// the item is the pair's first split.  Each wave finds it by itself among 64
-// sequences at a time; more are summed up first, 64 at a time, by every wave.
+// the item is the pair's first split.  Up to 64 sequences with the rows behind the last: each wave
+// finds it by itself among them.
 template <int ROWS, int KEYS, bool PAIRS>
 __device__ Item find_item(const PagedAttnArgs& a, int index) {
 #pragma clang fp contract(off)  // (the kernels of a call have to agree on the plan)
   if (a.plan != nullptr) return find_planned<ROWS, KEYS, PAIRS>(a, index);
-  const int lane = threadIdx.x & 63, B1 = a.p.B + 1;
+  const int lane = threadIdx.x & 63;
   Seq s{};
-  if (lane < B1) s = seq_of<ROWS, KEYS>(a, lane);
-  float work = static_cast<float>(s.tiles) * static_cast<float>(s.blocks);
-  if (a.target > 0)
-    for (int b = lane + 64; b < B1; b += 64) {
-      const Seq x = seq_of<ROWS, KEYS>(a, b);
-      work += static_cast<float>(x.tiles) * static_cast<float>(x.blocks);
-    }
-  int chunk = chunk_of(a, last_lane(wave_scan(work)));
-  // The card takes `one_round` items of a kv head at once: items just beyond a round take a whole
-  // one more, and each has a cost of its own.  If it is more than a round, of the splits 1, 1 1/8, .. 8 7/8
-  // times as long, one a lane, the one with the least rounds times blocks is taken (by
-  // estimate: products with reciprocals).
-  if (a.target > 0 && B1 <= 64) {  // (chunk < 2^26)
-    const float round = __builtin_amdgcn_rcpf(static_cast<float>(a.one_round));
-    auto splits = [&](int tiles, int blocks, float of) __attribute__((always_inline)) {
-      return static_cast<float>(tiles) * fmaxf(ceilf(static_cast<float>(blocks) * of - 1e-3f), 1.f);
-    };
-    if (last_lane(wave_scan(splits(s.tiles, s.blocks, __builtin_amdgcn_rcpf(static_cast<float>(chunk))))) * round > 1.001f) {
-      const int c = chunk + chunk / 8 * lane + chunk % 8 * lane / 8;
-      const float of = __builtin_amdgcn_rcpf(static_cast<float>(c));
-      float items = 0.f;
-      for (uint64_t left = __ballot(s.tiles > 0); left != 0; left &= left - 1) {
-        const int l = __builtin_ctzll(left);
-        items += splits(__builtin_amdgcn_readlane(s.tiles, l), __builtin_amdgcn_readlane(s.blocks, l), of);
-      }
-      const float cost = ceilf(items * round - 1e-3f) * static_cast<float>(c + a.item_cost);
-      chunk = __builtin_amdgcn_readlane(c, __builtin_ctzll(__ballot(cost == last_lane(wave_least(cost)))));
+  if (lane <= a.p.B) s = seq_of<ROWS, KEYS>(a, lane);
+  int chunk = chunk_of(a, last_lane(wave_scan(static_cast<float>(s.tiles) * static_cast<float>(s.blocks))));
+  if (a.target > 0) {  // (chunk < 2^26)
+    const float items = last_lane(wave_scan(items_by(s.tiles, s.blocks, __builtin_amdgcn_rcpf(static_cast<float>(chunk)))));
+    if (items > static_cast<float>(a.one_round) + 0.5f) {
+      const int c = longer(chunk, lane);
+      chunk = best_of(a, c, weigh_wave(s, c));
     }
   }
-  Count before{0, 0};
-  for (int b0 = 0; b0 < B1; b0 += 64) {
-    if (b0 > 0) {
-      s = Seq{};
-      if (b0 + lane < B1) s = seq_of<ROWS, KEYS>(a, b0 + lane);
-    }
-    const int splits = splits_of(s, chunk);
-    const Count mine = count_of(s, splits);
-    const int pairs = wave_scan(mine.pairs);
-    const uint32_t split = a.target > 0 ? static_cast<uint32_t>(wave_scan(static_cast<int>(mine.split))) : 0u;
-    const int first_pair = before.pairs + pairs - mine.pairs;
-    const uint32_t first_split = before.split + split - mine.split;
-    const int first = PAIRS ? first_pair : first_pair + static_cast<int>(first_split >> 16);
-    const uint64_t here = __ballot(index >= first && index - first < s.tiles * (PAIRS ? 1 : splits));
-    if (here != 0) {
-      const int l = __builtin_ctzll(here);
-      auto get = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
-      const Seq found{get(s.n), get(s.t0), get(s.len), get(s.keys), get(s.tiles), get(s.blocks)};
-      return item_of<PAIRS>(a, b0 + l, found, index - get(first), get(splits), chunk, static_cast<uint32_t>(get(static_cast<int>(first_split))));
-    }
-    before.pairs += last_lane(pairs);
-    before.split += static_cast<uint32_t>(last_lane(static_cast<int>(split)));
+  const int splits = splits_of(s, chunk);
+  const Count mine = count_of(s, splits);
+  const int first_pair = wave_scan(mine.pairs) - mine.pairs;
+  const uint32_t first_split = a.target > 0 ? static_cast<uint32_t>(wave_scan(static_cast<int>(mine.split))) - mine.split : 0u;
+  const int first = PAIRS ? first_pair : first_pair + static_cast<int>(first_split >> 16);
+  const uint64_t here = __ballot(index >= first && index - first < s.tiles * (PAIRS ? 1 : splits));
+  if (here == 0) {
+    Item none;
+    none.b = -1;
+    return none;
   }
-  Item none;
-  none.b = -1;
-  return none;
+  const int l = __builtin_ctzll(here);
+  auto get = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+  const Seq found{get(s.n), get(s.t0), get(s.len), get(s.keys), get(s.tiles), get(s.blocks)};
+  return item_of<PAIRS>(a, l, found, index - get(first), get(splits), chunk, static_cast<uint32_t>(get(static_cast<int>(first_split))));
 }
 
 constexpr int kPlanThreads = 1024;
@@ -362,6 +356,7 @@ template <int ROWS, int KEYS>
 __device__ void make_plan(const PagedAttnArgs& a) {
 #pragma clang fp contract(off)
   __shared__ float sums[kPlanThreads / 64];
+  __shared__ float weighed[kPlanThreads / 64][64];
   __shared__ Count ends[kPlanThreads / 64];
   PlanEntry* plan = static_cast<PlanEntry*>(a.plan);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, B1 = a.p.B + 1;
@@ -376,7 +371,22 @@ __device__ void make_plan(const PagedAttnArgs& a) {
   __syncthreads();
   work = 0.f;
   for (int w = 0; w < kPlanThreads / 64; ++w) work += sums[w];
-  const int chunk = chunk_of(a, work);
+  int chunk = chunk_of(a, work);
+  if (a.target > 0) {
+    const int c = longer(chunk, lane);
+    float items = 0.f;
+    for (int b0 = 0; b0 < B1; b0 += kPlanThreads) {
+      const int b = b0 + static_cast<int>(threadIdx.x);
+      Seq s{};
+      if (b < B1) s = seq_of<ROWS, KEYS>(a, b);
+      items += weigh_wave(s, c);
+    }
+    weighed[wave][lane] = items;
+    __syncthreads();
+    items = 0.f;
+    for (int w = 0; w < kPlanThreads / 64; ++w) items += weighed[w][lane];
+    chunk = best_of(a, c, items);
+  }
   Count before{0, 0};
   for (int b0 = 0; b0 < B1; b0 += kPlanThreads) {
     const int b = b0 + static_cast<int>(threadIdx.x);
@@ -1323,7 +1333,7 @@ size_t part_bytes(const PagedAttnArgs& a, int rows) {
 int tile_units(const PagedAttnArgs& a) { return a.d <= 64 ? 3 : 1; }
 
 // Sequences from which on a plan is made
-constexpr int kPlanned = 128;
+constexpr int kPlanned = 64;  // (find_item: a lane for each, and the rows behind the last)
 size_t plan_bytes(const PagedAttnArgs& a) { return (static_cast<size_t>(a.p.B) + 2) * sizeof(PlanEntry); }
 
 constexpr int kAllRows = 0x7fffffff;
@@ -1353,16 +1363,17 @@ Plan plan_of(PagedAttnArgs a) {
   else
     p.tile = a.p.T != a.p.B && rows > tile_rows(a);
   p.stream = !p.tile || a.p.B > 1;
-  // The stream form always splits: a sequence much longer than the others is spread over the card.  Up to
-  // 8 items a compute unit, where its workgroups are alone (60 single tokens after 8192: 362 us, from 2 a unit on 516 us, as
-  // 480 items are nearly a round already), of which the rounds decide (8 tokens after 4096: 35 us, always 8 a unit 48 us;
-  // 1 after 131072: 105 us and 125 us; 24 after 2048 to 16384, 4 heads: 102 us and 112 us).
-  const int per_cu = p.tile ? 2 * tile_units(a) : a.type == AttnType::kF32 ? 3 : 8;
+  // The stream form always splits: a sequence much longer than the others is spread over the card.  Up to 6 items a
+  // compute unit, of which the rounds decide (60 single tokens after 8192: 362 us, always 2 a unit 516 us, as
+  // 480 items are nearly a round already; 8 after 4096: 35 us, always 8 a unit 48 us; 1 after 131072: 105 and
+  // 125 us; 64 after 1024: 54 and 70 us).  One workgroup of 256 columns fills a unit's registers, and each has
+  // twice the rows to join: 2 (64 single tokens after 2048, 4 heads: 110 us, 192 us by 8; 128 us by 3).
+  const int per_cu = p.tile ? 2 * tile_units(a) : a.type == AttnType::kF32 ? 3 : a.d > 128 ? 2 : 6;
   const int64_t pairs = p.tile ? static_cast<int64_t>(a.p.B) + 1 : pairs_bound(a, kRows);  // (with the tile form: one a sequence)
   p.s = part_of(a, kRows, pairs, 0, p.tile ? kStreamRows : kAllRows, per_cu * kCus, p.tile ? 8 : 4);
-  const int units = p.tile ? tile_units(a) : a.type == AttnType::kF32 && a.d > 64 ? 1 : 2;
+  const int units = p.tile ? tile_units(a) : a.d > (a.type == AttnType::kF32 ? 64 : 128) ? 1 : 2;
   p.s.one_round = (units * kCus + a.hkv - 1) / a.hkv;
-  p.s.item_cost = a.type == AttnType::kF32 ? 6 : 16;
+  p.s.item_cost = a.type == AttnType::kF32 ? 6 : 12;
   // The tile form splits where whole tiles do not fill the card (1300 tokens after 8192, 168 tiles: 212 us,
   // 317 us whole; 3600 tokens after 16384, 456 tiles: 852 us, 1065 us if those split too: a
   // split's rows go through memory twice).  Splits of less than 8 blocks cost more than they give
