@@ -355,50 +355,63 @@ constexpr int kPlanThreads = 1024;
 template <int ROWS, int KEYS>
 __device__ void make_plan(const PagedAttnArgs& a) {
 #pragma clang fp contract(off)
-  __shared__ float sums[kPlanThreads / 64];
-  __shared__ float weighed[kPlanThreads / 64][64];
-  __shared__ Count ends[kPlanThreads / 64];
+  constexpr int kWaves = kPlanThreads / 64;
+  __shared__ float sums[kWaves];
+  __shared__ float weighed[kWaves][64];
+  __shared__ int tiles[kPlanThreads], blocks[kPlanThreads];
+  __shared__ Count ends[kWaves];
   PlanEntry* plan = static_cast<PlanEntry*>(a.plan);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, B1 = a.p.B + 1;
+  // (a sequence a thread is kept from loop to loop)
+  auto load = [&](int b) {
+    Seq s{};
+    if (b < B1) s = seq_of<ROWS, KEYS>(a, b);
+    return s;
+  };
+  const Seq mine0 = load(threadIdx.x);
+  auto seq_at = [&](int b0) { return b0 == 0 ? mine0 : load(b0 + static_cast<int>(threadIdx.x)); };
   float work = 0.f;
   if (a.target > 0)
-    for (int b = threadIdx.x; b < B1; b += kPlanThreads) {
-      const Seq s = seq_of<ROWS, KEYS>(a, b);
+    for (int b0 = 0; b0 < B1; b0 += kPlanThreads) {
+      const Seq s = seq_at(b0);
       work += static_cast<float>(s.tiles) * static_cast<float>(s.blocks);
     }
   work = wave_scan(work);
   if (lane == 63) sums[wave] = work;
   __syncthreads();
   work = 0.f;
-  for (int w = 0; w < kPlanThreads / 64; ++w) work += sums[w];
+  for (int w = 0; w < kWaves; ++w) work += sums[w];
   int chunk = chunk_of(a, work);
   if (a.target > 0) {
     const int c = longer(chunk, lane);
+    const float of = __builtin_amdgcn_rcpf(static_cast<float>(c));
     float items = 0.f;
-    for (int b0 = 0; b0 < B1; b0 += kPlanThreads) {
-      const int b = b0 + static_cast<int>(threadIdx.x);
-      Seq s{};
-      if (b < B1) s = seq_of<ROWS, KEYS>(a, b);
-      items += weigh_wave(s, c);
+    for (int b0 = 0; b0 < B1; b0 += kPlanThreads) {  // (every wave takes some of the sequences)
+      const Seq s = seq_at(b0);
+      __syncthreads();
+      tiles[threadIdx.x] = s.tiles;
+      blocks[threadIdx.x] = s.blocks;
+      __syncthreads();
+      for (int i = wave; i < min(B1 - b0, kPlanThreads); i += kWaves)
+        if (tiles[i] > 0) items += items_by(tiles[i], blocks[i], of);
     }
     weighed[wave][lane] = items;
     __syncthreads();
     items = 0.f;
-    for (int w = 0; w < kPlanThreads / 64; ++w) items += weighed[w][lane];
+    for (int w = 0; w < kWaves; ++w) items += weighed[w][lane];
     chunk = best_of(a, c, items);
   }
   Count before{0, 0};
   for (int b0 = 0; b0 < B1; b0 += kPlanThreads) {
     const int b = b0 + static_cast<int>(threadIdx.x);
-    Seq s{};
-    if (b < B1) s = seq_of<ROWS, KEYS>(a, b);
+    const Seq s = seq_at(b0);
     const Count mine = count_of(s, splits_of(s, chunk));
     const int pairs = wave_scan(mine.pairs);
     const uint32_t split = static_cast<uint32_t>(wave_scan(static_cast<int>(mine.split)));
     if (lane == 63) ends[wave] = {pairs, split};
     __syncthreads();
     Count here = before;
-    for (int w = 0; w < kPlanThreads / 64; ++w) {
+    for (int w = 0; w < kWaves; ++w) {
       if (w < wave) {
         here.pairs += ends[w].pairs;
         here.split += ends[w].split;

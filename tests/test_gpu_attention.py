@@ -523,6 +523,32 @@ def test_captured_batches_of_any_kind(ops):
         out.fill_(7.0)
 
 
+def test_captured_batch_of_many_sequences(ops):
+    """as above with more sequences than a wave has lanes: slots that fill up, one long one among them"""
+    count = 100
+    s = ref.batch([2] * count, [40] * count, 8, 2, 64, 16, torch.bfloat16, "cuda")
+    pool = torch.randn(400, 2, 16, 64, device="cuda").bfloat16()
+    s.update(kc=pool, vc=torch.randn_like(pool), table=torch.randint(0, 400, (count, 200), device="cuda", dtype=torch.int32))
+    graph = torch.cuda.CUDAGraph()
+    attend(ops, s)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = attend(ops, s)
+    for i in range(4):
+        new = [(1, 0, 1, 2)[(b + i) % 4] for b in range(count)]
+        new[i * 30] = 90
+        kv = [n + (b * 17 + i) % 60 for b, n in enumerate(new)]
+        kv[5 + i] += 3000
+        s["cu"].copy_(ints(0, *torch.tensor(new).cumsum(0).tolist()))
+        s["lens"].copy_(ints(*kv))
+        graph.replay()
+        want = attend(ops, {**s, "cu": s["cu"].clone(), "lens": s["lens"].clone()})
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+        check(ops, s)
+        out.fill_(7.0)
+
+
 def test_captured_gradient(ops):
     """forward and backward of the norm in one graph, replayed over new inputs"""
     torch.manual_seed(9)
