@@ -184,9 +184,9 @@ struct IrBlockF32Args {
   // reduce kernel (spread form below by default; NNSX_F32_IRW_INLAUNCH=1: the
   // last part of a tile to finish adds all slabs)
   int* tickets = nullptr;
-  // spread = 1: every part of a tile waits at a per-tile arrival counter (64-bit,
-  // monotone: tickets[] read as uint64) and then adds its 1/parts share of the
-  // tile's outputs from all slabs -- the combine spread over the parts, not left
+  // spread = 1: every part of a tile waits at a per-tile counter (tickets[] read as
+  // uint64: arrivals, departures; zero again after the launch) and then adds its
+  // 1/parts share of the tile's outputs from all slabs -- the combine spread over the parts, not left
   // to the last one.  Only launched when every workgroup of the grid is resident
   // at once (the host checks occupancy); the wait is bounded.
   int spread = 0;

@@ -235,6 +235,41 @@ def test_ir_block_f32_inlaunch_combine(nns, H, cin, hid, cout, stride, B):
     _close(ref, _ir_ref64(x, we, be, wd, bd, wp, bp, stride, cout, True, res), tol=5e-5)
 
 
+@pytest.mark.parametrize("H,cin,hid,cout,stride", [(56, 24, 144, 24, 1), (56, 24, 144, 32, 2), (28, 32, 192, 32, 1),
+                                                    (28, 32, 192, 64, 2), (14, 96, 576, 96, 1), (7, 160, 960, 160, 1)])
+@pytest.mark.parametrize("x3", [False, True])
+def test_ir_block_f32_one_ticket_buffer_for_batches_of_any_size(nns, H, cin, hid, cout, stride, x3):
+    """The number of hidden parts follows the batch (56x56: 3 at batch 2, 2 at batch 4), the ticket
+    buffer is the model's one: each launch leaves it zeroed, so the next may have other parts.
+    Bit for bit the separate reduce launch's sums."""
+    torch.manual_seed(H + cin)
+    we = torch.randn(hid, cin, device="cuda") / cin ** 0.5
+    be = torch.randn(hid, device="cuda") * 0.1
+    wd = torch.randn(9, hid, device="cuda") / 3
+    bd = torch.randn(hid, device="cuda") * 0.1
+    npad = (cout + 15) // 16 * 16
+    wp = torch.zeros(npad, hid, device="cuda")
+    wp[:cout] = torch.randn(cout, hid, device="cuda") / hid ** 0.5
+    bp = torch.zeros(npad, device="cuda")
+    bp[:cout] = torch.randn(cout, device="cuda") * 0.1
+    split = [None, None]
+    if x3:
+        for i, (w, rows, cols) in enumerate(((we, hid, (cin + 31) // 32 * 32), (wp[:cout], (cout + 31) // 32 * 32, hid))):
+            p = torch.zeros(rows, cols, device="cuda")
+            p[:w.shape[0], :w.shape[1]] = w
+            hi = p.bfloat16()
+            mid = (p - hi.float()).bfloat16()
+            split[i] = torch.stack([hi, mid, (p - hi.float() - mid.float()).bfloat16()]).contiguous()
+    res = stride == 1 and cin == cout
+    tickets = torch.zeros(768, dtype=torch.int32, device="cuda")
+    x = torch.randn(16, H, H, cin, device="cuda")
+    for B in (2, 4, 1, 8, 3, 16, 4, 2):
+        a = (x[:B], we, be, wd, bd, wp, bp, stride, cout, True, res, 1)
+        want = torch.ops.nnsx.ir_block(*a, None, *split)
+        assert torch.equal(torch.ops.nnsx.ir_block(*a, tickets, *split), want), B
+        assert int(tickets.count_nonzero()) == 0, B
+
+
 @pytest.mark.parametrize("skip", ["7,8,9", "6", "0,1,2,3,4"])
 def test_irw_tile_variants(skip):
     """The A/B tile configurations of the fused block (7 x 14 tiles on the
