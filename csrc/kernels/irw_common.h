@@ -103,7 +103,7 @@ __device__ __forceinline__ void irw_inlaunch_combine(const IrBlockF32Args& a, fl
   // fence either) and adds them in part order, + bias (+ residual) -- the sums
   // of irw_reduce in its order, without its launch -- then resets the ticket
   // for the next launch (tickets start at zero: the caller's buffer is zeroed
-  // once at creation, and every launch leaves it so).  Correct for any placement of the parts over XCDs.
+  // once at creation).  Correct for any placement of the parts over XCDs.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();  // every wave's slab stores done; the LDS is free
   const int64_t plane = static_cast<int64_t>(a.B) * a.Ho * a.Wo * a.cout;
@@ -129,35 +129,34 @@ __device__ __forceinline__ void irw_inlaunch_combine(const IrBlockF32Args& a, fl
     }
   };
   if (a.spread) {
-    // spread form: one lane per part counts its arrival in the low half of the
-    // tile's 64-bit counter and waits until all parts of this launch have
-    // arrived; then each part adds its 1/nparts share.  Past the wait it counts
-    // its departure in the high half, and the part that departs last sets the
-    // counter back to zero: nobody reads it any more, and the next launch starts
-    // from zero whatever its number of parts is.  (A count that only grows has to be
-    // a multiple of nparts at the start, which a buffer used at batch 2 -- 3 parts
-    // on the 56 x 56 blocks -- and then at batch 4 -- 2 parts -- is not: half of the
-    // parts went on before the others' slabs were there, the rest ran into the bound.)
+    // spread form: one lane per part adds its share of kSpreadRound to the tile's
+    // 64-bit arrival count and waits until the count reaches the next multiple
+    // of it, which is when every part of this launch has arrived; then each
+    // part adds its 1/nparts share of the sums.  The shares of a launch add up to the whole
+    // whatever its number of parts is, so every launch starts at a multiple. (A
+    // count of parts has to be a multiple of nparts at the start, which that of a
+    // buffer used at batch 2 -- 3 parts on the 56 x 56 blocks -- and then at batch 4
+    // -- 2 parts -- is not: half of the parts went on before the others' slabs
+    // were there, the rest ran into the bound.  Zeroing the count after each
+    // launch takes one more atomic a part: batch 1 286 us a forward, 270 this way.)
     // The host launches this form only when the whole grid is resident at
     // once; the wait is bounded all the same (~0.2 s), so a broken residency
     // assumption shows up as wrong sums, never as a hung GPU.
-    unsigned long long* ctr = reinterpret_cast<unsigned long long*>(a.tickets) + tile;
-    unsigned departed = 0;
     if (tid == 0) {
-      __hip_atomic_fetch_add(ctr, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      for (int it = 0; it < (1 << 21); ++it) {
-        if (static_cast<int>(__hip_atomic_load(ctr, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) >= nparts) break;
+      unsigned long long* ctr = reinterpret_cast<unsigned long long*>(a.tickets) + tile;
+      const unsigned long long share = part == 0 ? a.spread_first : a.spread;
+      unsigned long long now = __hip_atomic_fetch_add(ctr, share, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const unsigned long long target = (now / kSpreadRound + 1) * kSpreadRound;
+      now += share;  // (the last to arrive need not look)
+      for (int it = 0; now < target && it < (1 << 21); ++it) {
         __builtin_amdgcn_s_sleep(2);
+        now = __hip_atomic_load(ctr, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
-      departed = static_cast<unsigned>(
-          __hip_atomic_fetch_add(ctr, 1ull << 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) >> 32);
     }
     __syncthreads();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");  // (no instruction: keeps the loads below the wait)
     const int total = TY * TX * nq, chunk = (total + nparts - 1) / nparts;
     combine(part * chunk, min(total, (part + 1) * chunk));
-    if (tid == 0 && departed == static_cast<unsigned>(nparts - 1))  // (used here: its way back is hidden by the sums)
-      __hip_atomic_store(ctr, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     return;
   }
   int* flag = reinterpret_cast<int*>(smem);

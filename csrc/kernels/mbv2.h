@@ -160,6 +160,10 @@ void avgpool_f32(const float* x, float* y, int B, int HW, int C, hipStream_t s);
 void pw_pool_f32(const float* x, const float* wt, const float* bias, float* y, int B, int HW, int N, int K, int Kpad,
                  int Npad, int act, hipStream_t s, X3W w3 = X3W{});
 
+// what a launch adds to a tile's arrival count (IrBlockF32Args::spread): more than any
+// number of parts; a count lasts for 2^48 launches
+constexpr int kSpreadRound = 1 << 16;
+
 // fused inverted residual, fp32.  we [hid][KIN] (KIN = ceil8(cin), zero
 // padded), wd [9][hid], wp [ceil16(cout)][hid] (rows zero padded); biases
 // [hid] / [hid] / [ceil16(cout)].
@@ -184,12 +188,13 @@ struct IrBlockF32Args {
   // reduce kernel (spread form below by default; NNSX_F32_IRW_INLAUNCH=1: the
   // last part of a tile to finish adds all slabs)
   int* tickets = nullptr;
-  // spread = 1: every part of a tile waits at a per-tile counter (tickets[] read as
-  // uint64: arrivals, departures; zero again after the launch) and then adds its
-  // 1/parts share of the tile's outputs from all slabs -- the combine spread over the parts, not left
+  // spread > 0: every part of a tile waits at a per-tile arrival count (tickets[] read as
+  // uint64) and then adds its 1/parts share of the
+  // tile's outputs from all slabs -- the combine spread over the parts, not left
   // to the last one.  Only launched when every workgroup of the grid is resident
-  // at once (the host checks occupancy); the wait is bounded.
-  int spread = 0;
+  // at once (the host checks occupancy); the wait is bounded.  A part adds `spread` to the count,
+  // the first one spread_first: a launch kSpreadRound in all, whatever its number of parts
+  int spread = 0, spread_first = 0;
   // split-bf16 weights (F32Math::kX3): we3 [3][hid][ceil32(cin)], wp3
   // [3][ceil32(cout)][hid] bf16 (hi, mid, lo parts; zero padded).  Both set and
   // the method x3: the irw_x3 kernel of the same geometry, when there is one

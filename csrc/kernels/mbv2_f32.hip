@@ -2078,7 +2078,7 @@ static bool irw_atomic2() { return false; }
 
 // NNSX_F32_IRW_INLAUNCH: 0 = irw_reduce launch, 1 = last-arriver combine,
 // 2 = spread combine (default: every part waits for its tile's other parts,
-// then adds a 1/parts share; 64-bit counters: two int32 ticket
+// then adds a 1/parts share; 64-bit monotone counters: two int32 ticket
 // entries per tile).  Batch 1 at a 500 fps live camera: filter device time
 // 317-319 vs 329-335 us, p50 356-363 vs 368-383 us with the reduce launches
 // (profiles/r3_b1_launch_count_ab.txt); back-to-back replays are unchanged.
@@ -2099,7 +2099,7 @@ bool set_device_shared(bool on) {
 
 // the model's ticket buffer (ir_block_f32_tickets ints, zeroed once): the
 // spread form's 64-bit counters in [0, kSpreadTickets), the last-arriver
-// form's ints after them (kLastTickets); either form leaves zeros.  Hidden parts > 1 only
+// form's self-resetting ints after them (kLastTickets).  Hidden parts > 1 only
 // below 256 tiles (irw_parts), so both regions hold every splitting launch.
 constexpr int kSpreadTickets = 512, kLastTickets = 256;
 
@@ -2170,15 +2170,18 @@ static bool launch_irw(const IrwCfg* c, IrBlockF32Args a, hipStream_t s) {
         hipDeviceGetAttribute(&ncu, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess &&
         hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, reinterpret_cast<const void*>(c->kernel), 64 * c->NW, lds) ==
             hipSuccess &&
-        static_cast<int64_t>(tiles) * a.hsplit <= static_cast<int64_t>(ncu) * std::max(1, per_cu - 1))
-      a.spread = 1;
-    else if (irw_inlaunch_mode() == 1 || a.hsplit <= 4)
-      // last-arriver form (int tickets, their own region of the buffer): a grid larger than
+        static_cast<int64_t>(tiles) * a.hsplit <= static_cast<int64_t>(ncu) * std::max(1, per_cu - 1)) {
+      a.spread = kSpreadRound / a.hsplit;
+      a.spread_first = kSpreadRound - (a.hsplit - 1) * a.spread;
+    } else if (irw_inlaunch_mode() == 1 || a.hsplit <= 4) {
+      // last-arriver form (self-resetting int tickets, their own region of the
+      // buffer: the spread form's counters there only grow): a grid larger than
       // the chip -- DeepLab's 33x33 blocks at batch 8, 200 tiles x 2 parts --
       // has few slabs per tile, so the last part adds them alone cheaply
       a.tickets += kSpreadTickets;
-    else
+    } else {
       a.tickets = nullptr;  // (separate reduce launch: many slabs, spread over its grid)
+    }
   }
   hipLaunchKernelGGL(c->kernel, dim3(static_cast<unsigned>(tiles * a.hsplit)), dim3(64 * c->NW), lds, s, a);
   if (a.ws && !a.tickets) {

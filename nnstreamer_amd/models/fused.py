@@ -151,7 +151,7 @@ class Block(nn.Module):
         self.cin = cin
         self.cout = int(p[0].out_channels)
         # tickets of the fp32 kernel's in-launch combine of hidden-channel parts
-        # (small batches): zero here, and every launch leaves them zero again
+        # (small batches): zero here; a launch leaves what the next can start from
         self.register_buffer("ir_tickets", torch.zeros(768 if self.f32 else 1, dtype=torch.int32))
         if self.f32:
             self._init_f32(cin, hid)
