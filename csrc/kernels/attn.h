@@ -43,6 +43,7 @@ struct PagedAttnArgs {
   // derived by the launcher: rows a token, and how the keys are split (attn.hip, plan)
   int group = 1, target = 0, min_chunk = 1, slots = 0, pairs = 0, parts = 0, apart = 1, one_round = 0, item_cost = 0, rows_lo = 0, rows_hi = 0;
   void* plan = nullptr;
+  int* chunk = nullptr;  // key blocks of a split, left by the attention for the join
 };
 // bytes of scratch memory the call needs (0: none)
 size_t paged_attn_workspace_bytes(const PagedAttnArgs& a);

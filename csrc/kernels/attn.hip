@@ -317,20 +317,25 @@ __device__ __forceinline__ int best_of(const PagedAttnArgs& a, int chunk, float 
 
 // PAIRS false: `index` counts items; PAIRS true: (sequence, tile) pairs, and
 // the item is the pair's first split.  Up to 64 sequences with the rows behind the last: each wave
-// finds it by itself among them.
+// finds it by itself among them.  The split comes from sums of floats, which another kernel's code might round
+// otherwise (products fused into sums or not): the join takes the one that the attention has left in a.chunk.
 template <int ROWS, int KEYS, bool PAIRS>
 __device__ Item find_item(const PagedAttnArgs& a, int index) {
-#pragma clang fp contract(off)  // (the kernels of a call have to agree on the plan)
   if (a.plan != nullptr) return find_planned<ROWS, KEYS, PAIRS>(a, index);
   const int lane = threadIdx.x & 63;
   Seq s{};
   if (lane <= a.p.B) s = seq_of<ROWS, KEYS>(a, lane);
-  int chunk = chunk_of(a, last_lane(wave_scan(static_cast<float>(s.tiles) * static_cast<float>(s.blocks))));
-  if (a.target > 0) {  // (chunk < 2^26)
-    const float items = last_lane(wave_scan(items_by(s.tiles, s.blocks, __builtin_amdgcn_rcpf(static_cast<float>(chunk)))));
-    if (items > static_cast<float>(a.one_round) + 0.5f) {
-      const int c = longer(chunk, lane);
-      chunk = best_of(a, c, weigh_wave(s, c));
+  int chunk;
+  if constexpr (PAIRS) {
+    chunk = *a.chunk;
+  } else {
+    chunk = chunk_of(a, last_lane(wave_scan(static_cast<float>(s.tiles) * static_cast<float>(s.blocks))));
+    if (a.target > 0) {  // (chunk < 2^26)
+      const float items = last_lane(wave_scan(items_by(s.tiles, s.blocks, __builtin_amdgcn_rcpf(static_cast<float>(chunk)))));
+      if (items > static_cast<float>(a.one_round) + 0.5f) {
+        const int c = longer(chunk, lane);
+        chunk = best_of(a, c, weigh_wave(s, c));
+      }
     }
   }
   const int splits = splits_of(s, chunk);
@@ -342,6 +347,7 @@ __device__ Item find_item(const PagedAttnArgs& a, int index) {
   if (here == 0) {
     Item none;
     none.b = -1;
+    none.chunk = chunk;
     return none;
   }
   const int l = __builtin_ctzll(here);
@@ -354,7 +360,6 @@ constexpr int kPlanThreads = 1024;
 
 template <int ROWS, int KEYS>
 __device__ void make_plan(const PagedAttnArgs& a) {
-#pragma clang fp contract(off)
   constexpr int kWaves = kPlanThreads / 64;
   __shared__ float sums[kWaves];
   __shared__ float weighed[kWaves][64];
@@ -491,6 +496,7 @@ __device__ __forceinline__ void stream_item(const PagedAttnArgs& a, unsigned ind
   const int head = static_cast<int>(index % a.hkv);
   const int slot = static_cast<int>(index / a.hkv);
   const Item it = find_item<kRows, kKeys, false>(a, slot);
+  if (index == 0 && threadIdx.x == 0 && a.chunk != nullptr) *a.chunk = it.chunk;
   if (it.b < 0) return;
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -850,6 +856,7 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, unsigned index
   const int head = static_cast<int>(index % a.hkv);
   const int slot = static_cast<int>(index / a.hkv);
   const Item it = find_item<ROWS, kTileKeys, false>(a, slot);
+  if (index == 0 && threadIdx.x == 0 && a.chunk != nullptr) *a.chunk = it.chunk;
   if (it.b < 0) return;
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1403,9 +1410,13 @@ Plan plan_of(PagedAttnArgs a) {
   p.t.ws = ws;
   ws += p.tile ? part_bytes(p.t, tile_rows(a)) : 0;
   p.s.plan = p.t.plan = nullptr;
+  p.s.chunk = p.t.chunk = nullptr;
   if (a.p.B >= kPlanned) {
     if (p.stream) p.s.plan = ws;
     if (p.tile) p.t.plan = ws + plan_bytes(a);
+  } else {
+    if (p.stream && p.s.target > 0) p.s.chunk = reinterpret_cast<int*>(ws);
+    if (p.tile && p.t.target > 0) p.t.chunk = reinterpret_cast<int*>(ws) + 1;
   }
   return p;
 }
@@ -1462,8 +1473,8 @@ void launch(const Plan& p, hipStream_t s) {
 
 size_t paged_attn_workspace_bytes(const PagedAttnArgs& a) {
   const Plan p = plan_of(a);
-  return (p.stream ? part_bytes(p.s, kRows) : 0) + (p.tile ? part_bytes(p.t, tile_rows(a)) : 0) +
-         (a.p.B >= kPlanned ? 2 * plan_bytes(a) : 0);
+  const size_t parts = (p.stream ? part_bytes(p.s, kRows) : 0) + (p.tile ? part_bytes(p.t, tile_rows(a)) : 0);
+  return parts + (a.p.B >= kPlanned ? 2 * plan_bytes(a) : parts > 0 ? 2 * sizeof(int) : 0);
 }
 
 void paged_attn(const PagedAttnArgs& a, hipStream_t s) {
