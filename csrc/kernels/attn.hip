@@ -142,6 +142,17 @@ __device__ __forceinline__ float row_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// Scores times `c` are rounded before their maximum is taken, but fused into the exponent's subtraction: the
+// largest key's exponent is off by half a step of the maximum.  From 2^20 on that may be more than 2^-4 (from 2^28 on
+// it would leave fp16's range), and the products are rounded first there too, so that it is 0.
+constexpr float kFar = 1048576.f;
+__device__ __forceinline__ bool any_far(float max) { return __any(fabsf(max) >= kFar && max != kNegInf); }
+__device__ __forceinline__ float far_exponent(float s, float c, float max, float lift) {
+  float x = s * c;
+  asm("" : "+v"(x));  // (a product by itself)
+  return x - max + lift;
+}
+
 // ------------------------------------------------------------------- plan ----
 // Work is cut into items: (sequence, tile of rows, split of its key blocks).
 // Lengths live on the device, so every wave derives its own item from them (of many
@@ -549,6 +560,7 @@ __device__ __forceinline__ void stream_item(const PagedAttnArgs& a, unsigned ind
 #pragma unroll
   for (int m = 0; m < NB; ++m) o[m] = (f32x16)(0.f);
   float mx = kNegInf, sum = 0.f;
+  bool distant = false;  // some row's maximum is
   const float c = a.scale * kLog2e, inf = opaque_infinity();
 
   u32x4 k[KC];
@@ -645,7 +657,7 @@ __device__ __forceinline__ void stream_item(const PagedAttnArgs& a, unsigned ind
     for (int i = 1; i < 16; ++i) bm = max2(bm, s[i], inf);
     bm = row_max(bm, inf);
     const float nm = fmaxf(mx, bm * c);
-    const float to = nm == kNegInf ? 0.f : nm, base = to - kLift<T>;  // (a row may have seen nothing yet)
+    const float to = nm == kNegInf ? 0.f : nm;  // (a row may have seen nothing yet)
     if (__any(nm > mx)) {
       const float f = __builtin_amdgcn_exp2f(mx - to);
       sum *= f;
@@ -654,10 +666,18 @@ __device__ __forceinline__ void stream_item(const PagedAttnArgs& a, unsigned ind
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[m][i] *= f;
       mx = nm;
+      distant = any_far(mx);
+    }
+    float by = c, base = to - kLift<T>;
+    if (distant) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = far_exponent(s[i], c, to, kLift<T>);
+      by = 1.f;
+      base = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      s[i] = __builtin_amdgcn_exp2f(s[i] * c - base);
+      s[i] = __builtin_amdgcn_exp2f(s[i] * by - base);
       sum += s[i];
     }
 
@@ -906,6 +926,7 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, unsigned index
 #pragma unroll
   for (int m = 0; m < NB; ++m) o[m] = (f32x16)(0.f);
   float mx = kNegInf, sum = 0.f;
+  int distant = 0;  // some row's maximum is
   const float c = a.scale * kLog2e, inf = opaque_infinity();
 
   if (a.p.pages == 0) blk1 = blk0;
@@ -1061,9 +1082,9 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, unsigned index
     for (int i = 1; i < 15; i += 2) bm = max3(bm, max2(s[0][i], s[1][i], inf), max2(s[0][i + 1], s[1][i + 1], inf));
     const float nm = fmaxf(mx, row_max(max2(bm, max2(s[0][15], s[1][15], inf), inf), inf) * c);
     // the maximum that weights are relative to follows only steps of more than
-    // 2^8: weights stay within [0, 2^15], inside every type's range, and the
+    // 2^8: weights stay within [0, 2^15 and a sixteenth], inside every type's range, and the
     // rescale of O is rare (8192 tokens, 32 heads of 128 columns: 580 us, 605 us with every step followed)
-    if (__any(nm > mx + 8.f)) {
+    if (__any(nm > mx + (distant ? 0.f : 8.f))) {
       const float f = __builtin_amdgcn_exp2f(mx - (nm == kNegInf ? 0.f : nm));
       sum *= f;
 #pragma unroll
@@ -1071,9 +1092,18 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, unsigned index
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[m][i] *= f;
       mx = nm;
+      distant = __builtin_amdgcn_readfirstlane(any_far(mx));
     }
     if (there != ~0ull || key0 < t_in_lo || key0 + kTileKeys > t_in_hi) take_infinite(v, key0, there);
-    const float base = (mx == kNegInf ? 0.f : mx) - kLift<T>;  // (a row may have seen nothing yet)
+    float by = c, base = (mx == kNegInf ? 0.f : mx) - kLift<T>;  // (a row may have seen nothing yet)
+    if (distant) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[b][i] = far_exponent(s[b][i], c, mx == kNegInf ? 0.f : mx, kLift<T>);
+      by = 1.f;
+      base = 0.f;
+    }
     u32x4 p[4];
     auto weigh = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
@@ -1081,7 +1111,7 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, unsigned index
         float w[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          w[h] = __builtin_amdgcn_exp2f(s[t / 2][8 * (t % 2) + 2 * e + h] * c - base);
+          w[h] = __builtin_amdgcn_exp2f(s[t / 2][8 * (t % 2) + 2 * e + h] * by - base);
           sum += w[h];
         }
         p[t][e] = pack2<T>(w[0], w[1]);

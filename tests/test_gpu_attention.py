@@ -263,6 +263,39 @@ def test_paged_attention_large_scores(ops):
     check(ops, s, scale=1e-3)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new,kv", [(1, 70), (2, 9000), (9, 3000), (200, 200), (150, 3000)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_paged_attention_scores_of_billions(ops, dtype, new, kv, dim):
+    """Finite scores up to 2^31, either sign: a row is the mean of the values whose keys have its largest score.
+    A score is one product of two values of 4 bits and less, so exact in fp32; two that differ do so by 2^19 at
+    least (2^15 times the smallest step of the keys, 2^4), so the smaller one's weight is 0, and that of the largest
+    is a power of two.  What is left: the sum of the values in fp32 and the rounding of the result."""
+    s = ref.batch([new], [kv], 4, 2, dim, 16, dtype, "cuda", stale=0.0)
+    gen = torch.Generator().manual_seed(new + kv)
+    size = 2.0 ** torch.randint(8, 16, (2, kv), generator=gen)
+    top = (torch.randint(8, 16, (2, kv), generator=gen) / 8 * size / 2).to(dtype).double()  # (4 bits each: many ties)
+    at = s["table"][0].cpu()[torch.arange(kv) // 16].long()
+    k = torch.zeros(kv, 2, dim, dtype=torch.float64)
+    k[:, :, 3] = top.t()
+    s["kc"][at.cuda(), :, (torch.arange(kv) % 16).cuda()] = k.to(dtype).cuda()
+    v = s["vc"][at.cuda(), :, (torch.arange(kv) % 16).cuda()].double().cpu()  # [kv, 2, dim]
+    s["q"].zero_()
+    sign = torch.tensor([1.0, -1.0, 1.0, -1.0])
+    s["q"][:, :, 3] = (sign * 2.0 ** 15).to(dtype).cuda()
+    for causal in (True, False):
+        got = attend(ops, s, scale=1.0, causal=causal).double().cpu()
+        pos = torch.arange(kv - new, kv)[:, None]
+        for h in range(4):
+            score = (sign[h] * k[:, h // 2, 3]).expand(new, kv)
+            if causal:
+                score = score.masked_fill(torch.arange(kv) > pos, float("-inf"))
+            w = (score == score.max(1, keepdim=True).values).double()
+            want = w @ v[:, h // 2] / w.sum(1, keepdim=True)
+            mag = w @ v[:, h // 2].abs() / w.sum(1, keepdim=True)
+            ref.close(got[:, h], want, mag * (w.sum(1, keepdim=True) + 8) * ref.F32 + want.abs() * ref.half_step(dtype) + ref.smallest(dtype))
+
+
 # ------------------------------------------------------- norm and rotation ----
 
 SHAPES = [(1, 1, 8, 8), (4, 2, 64, 64), (3, 3, 40, 16), (8, 1, 128, 128), (5, 5, 72, 72), (2, 1, 256, 128), (32, 8, 128, 128),
