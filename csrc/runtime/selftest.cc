@@ -25,6 +25,7 @@
 #include <thread>
 #include <vector>
 
+#include "core/util.h"
 #include "kernels/kernels.h"
 #include "runtime/hip_util.h"
 #include "runtime/memory.h"
@@ -97,28 +98,43 @@ std::string host_h2d(int dev, bool pinned) {
   return r;
 }
 
-// A stream whose work does not hold up `rs`: streams share a few hardware
-// queues, and a free ordered on rs would come after the spin of a stream in its
-// queue whatever it waits for.  Those tried before stay in `tried`, so that the next gets another queue.
-hipStream_t stream_beside(hipStream_t rs, int dev, std::vector<hipStream_t>* tried) {
-  hipEvent_t e = hip::event_get(dev);
-  hipStream_t s = nullptr;
-  for (int i = 0; i < 8; ++i) {
-    hip::check(hipStreamCreateWithFlags(&s, hipStreamNonBlocking), "selftest stream");
-    tried->push_back(s);
-    kernels::spin_us(s, 1);  // (its code is loaded)
-    hip::check(hipStreamSynchronize(s), "selftest sync");
-    kernels::spin_us(s, 4000);
-    hip::check(hipEventRecord(e, rs), "selftest event");
-    std::this_thread::sleep_for(std::chrono::milliseconds(1));
-    const bool passed = hipEventQuery(e) == hipSuccess && hipStreamQuery(s) != hipSuccess;
-    hip::check(hipStreamSynchronize(s), "selftest sync");
-    if (passed) break;
+// Streams of which the last one's work does not hold up `rs`: streams share a few
+// hardware queues, and a free ordered on rs would come after the spin of a stream in its
+// queue whatever it waits for.  Those tried before stay, so that the next gets another queue.
+// Throws where none of `tries` is beside it: a case run all the same would tell nothing.
+struct StreamBeside {
+  std::vector<hipStream_t> tried;
+  hipStream_t get() const { return tried.back(); }
+  StreamBeside(hipStream_t rs, int dev, int tries = 8) {
+    hipEvent_t e = hip::event_get(dev);
+    bool passed = false;
+    for (int i = 0; i < tries && !passed; ++i) {
+      hipStream_t s = nullptr;
+      hip::check(hipStreamCreateWithFlags(&s, hipStreamNonBlocking), "selftest stream");
+      tried.push_back(s);
+      kernels::spin_us(s, 1);  // (its code is loaded)
+      hip::check(hipStreamSynchronize(s), "selftest sync");
+      kernels::spin_us(s, 4000);
+      hip::check(hipEventRecord(e, rs), "selftest event");
+      std::this_thread::sleep_for(std::chrono::milliseconds(1));
+      passed = hipEventQuery(e) == hipSuccess && hipStreamQuery(s) != hipSuccess;
+      hip::check(hipStreamSynchronize(s), "selftest sync");
+    }
+    hip::check(hipStreamSynchronize(rs), "selftest sync");
+    hip::event_put(dev, e);
+    if (!passed) {
+      destroy();
+      throw Error("memory_selftest: no stream beside the release stream's hardware queue, nothing was tested");
+    }
   }
-  hip::check(hipStreamSynchronize(rs), "selftest sync");
-  hip::event_put(dev, e);
-  return s;
-}
+  ~StreamBeside() { destroy(); }
+  StreamBeside(const StreamBeside&) = delete;
+  StreamBeside& operator=(const StreamBeside&) = delete;
+  void destroy() {
+    for (hipStream_t s : tried) (void)hipStreamDestroy(s);
+    tried.clear();
+  }
+};
 
 // the mirror of a host memory is read on a second stream (spinning first),
 // which records its use on the HOST memory (what a filter's replay lane does);
@@ -131,10 +147,9 @@ std::string mirror_other_stream(int dev) {
   // free past the reader and hide the undone fix
   Memory::drain_deferred();
   hip::check(hipStreamSynchronize(hip::release_stream(dev)), "selftest sync");
-  hipStream_t s1 = nullptr;
+  const StreamBeside beside(hip::release_stream(dev), dev);
+  hipStream_t s1 = nullptr, s2 = beside.get();
   hip::check(hipStreamCreateWithFlags(&s1, hipStreamNonBlocking), "selftest stream");
-  std::vector<hipStream_t> tried;
-  hipStream_t s2 = stream_beside(hip::release_stream(dev), dev, &tried);
   // (pageable: its release does not wait for readers on the host -- the mirror's
   // own release must order itself after them)
   MemoryPtr h = Memory::alloc_host(kBytes);
@@ -183,7 +198,6 @@ std::string mirror_other_stream(int dev) {
   out.reset();
   hip::check(hipDeviceSynchronize(), "selftest sync");
   (void)hipStreamDestroy(s1);
-  for (hipStream_t s : tried) (void)hipStreamDestroy(s);
   return r;
 }
 
@@ -235,6 +249,11 @@ std::string memory_selftest(const std::string& name, int dev) {
   if (name == "pinned_h2d") return host_h2d(dev, true);
   if (name == "mirror_other_stream") return mirror_other_stream(dev);
   if (name == "device_reader") return device_reader(dev);
+  if (name == "no_stream_beside") {  // (what mirror_other_stream does where it cannot tell)
+    hip::DeviceGuard g(dev);
+    StreamBeside none(hip::release_stream(dev), dev, 0);
+    return "memory_selftest: ran without a stream";
+  }
   return "memory_selftest: unknown case " + name;
 }
 

@@ -51,6 +51,16 @@ def test_memory_selftest_fails_without_its_fix(nns, case, mutation, monkeypatch)
     assert _C.memory_selftest(case, 0) == ""
 
 
+def test_memory_selftest_without_a_stream_beside(nns):
+    """mirror_other_stream needs a stream of another hardware queue than the release
+    stream's: where none is found it says so instead of passing or failing by chance"""
+    from nnstreamer_amd import _C
+
+    with pytest.raises(RuntimeError, match="nothing was tested"):
+        _C.memory_selftest("no_stream_beside", 0)
+    assert _C.memory_selftest("mirror_other_stream", 0) == ""
+
+
 def test_pageable_h2d_without_its_fix_on_this_runtime(nns, monkeypatch, capfd):
     """The pageable half of 7ba8684 on this HIP runtime (ROCm 7.2): measured, a
     pageable H2D of <= 1 MB returns at once with the source already staged (the
