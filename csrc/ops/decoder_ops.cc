@@ -431,7 +431,9 @@ Angles angles(const at::Tensor& pos, const at::Tensor& rope) {
   at::Tensor p = pos.to(at::kLong);
   a.there = p.ge(0).logical_and(p.lt(rope.size(0)));
   p = p.masked_fill(a.there.logical_not(), 0);
-  const at::Tensor rows = rope.size(0) ? rope.index({p}) : at::zeros({p.size(0), rope.size(1)}, rope.options());
+  auto sizes = p.sizes().vec();
+  sizes.push_back(rope.size(1));
+  const at::Tensor rows = rope.size(0) ? rope.index({p}) : at::zeros(sizes, rope.options());
   a.cos = rows.slice(-1, 0, rope.size(1) / 2).unsqueeze(-2);
   a.sin = rows.slice(-1, rope.size(1) / 2).unsqueeze(-2);
   a.there = a.there.unsqueeze(-1).unsqueeze(-1);

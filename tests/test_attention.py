@@ -84,6 +84,17 @@ def test_qk_norm_rope_gradient_without_weights_and_second_order(ops):
         torch.autograd.grad(y[0].sum(), q, create_graph=True)
 
 
+def test_qk_norm_rope_empty_table(ops):
+    """no position is in a table of none: zero rows, zero gradients, whatever the positions' shape"""
+    for shape, positions in (((2, 3), torch.tensor([[0, 1, 2], [5, -1, 0]])), ((2, 3), torch.arange(3)), ((3,), torch.arange(3))):
+        q, k = (torch.randn(*shape, n, 16, requires_grad=True) for n in (4, 2))
+        w = torch.rand(16, requires_grad=True)
+        y = ops.qk_norm_rope(q, k, w, w, positions, ops.rope_table(0, 16))
+        assert y[0].shape == q.shape and y[1].shape == k.shape and not y[0].any() and not y[1].any()
+        d = torch.autograd.grad(y, [q, k, w], [torch.ones_like(q), torch.ones_like(k)])
+        assert [x.shape for x in d] == [q.shape, k.shape, w.shape] and not any(x.any() for x in d)
+
+
 BATCHES = [
     ([1], [1], 1, 1, 8, 4), ([1], [0], 2, 1, 8, 4), ([0], [5], 2, 1, 8, 4), ([5], [3], 2, 2, 16, 4),
     ([3, 0, 1, 6], [10, 4, 33, 6], 6, 2, 24, 3), ([2, 9], [70, 9], 4, 4, 32, 1), ([4, 1], [20, 64], 8, 1, 64, 16),

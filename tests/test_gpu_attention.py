@@ -323,6 +323,15 @@ def test_qk_norm_rope(ops, dtype, hq, hk, dim, rot, inter):
         ref.close(dw, want[2], want[3])
 
 
+def test_qk_norm_rope_empty_table(ops):
+    q, k = (torch.randn(2, 3, n, 16, device="cuda", requires_grad=True) for n in (4, 2))
+    w = torch.rand(16, device="cuda", requires_grad=True)
+    for pos in (torch.tensor([[0, 1, 2], [5, -1, 0]], device="cuda"), torch.arange(3, device="cuda")):
+        y = ops.qk_norm_rope(q, k, w, w, pos, ops.rope_table(0, 16).cuda())
+        d = torch.autograd.grad(y, [q, k, w], [torch.ones_like(q), torch.ones_like(k)])
+        assert [x.shape for x in d] == [q.shape, k.shape, w.shape] and not any(x.any() for x in (*y, *d))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_qk_norm_rope_views(ops, dtype):
     """views of a fused projection, broadcast positions of either type, fp32 weights, one weight
