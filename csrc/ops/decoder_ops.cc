@@ -653,14 +653,19 @@ struct QkNormRopeBackward : public torch::autograd::Node {
   }
 };
 
+// a tangent would be dropped unnoticed
+void no_forward_gradient(const char* op, std::initializer_list<const at::Tensor*> ts) {
+  for (const auto* t : ts)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), op, " has no forward-mode gradient");
+}
+
 std::tuple<at::Tensor, at::Tensor> qk_norm_rope_autograd(const at::Tensor& q, const at::Tensor& k, const OptTensor& qw,
                                                          const OptTensor& kw, const at::Tensor& pos,
                                                          const at::Tensor& rope, double eps, bool interleaved) {
   using torch::autograd::SavedVariable;
   TORCH_CHECK(!at::GradMode::is_enabled() || !rope.requires_grad(), "qk_norm_rope: no gradient for the table of angles");
   const at::Tensor wq = given(qw) ? *qw : at::Tensor(), wk = given(kw) ? *kw : at::Tensor();
-  for (const auto* t : {&q, &k, &wq, &wk})
-    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), "qk_norm_rope has no forward-mode gradient");
+  no_forward_gradient("qk_norm_rope", {&q, &k, &wq, &wk, &rope});
   std::shared_ptr<QkNormRopeBackward> node;
   if (torch::autograd::compute_requires_grad(q, k, wq, wk)) {
     node = std::shared_ptr<QkNormRopeBackward>(new QkNormRopeBackward, torch::autograd::deleteNode);
@@ -691,6 +696,7 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rope_autograd(const at::Tensor& q, co
 
 // an operator without a derivative says so where one would be recorded
 void no_gradient(const char* op, std::initializer_list<const at::Tensor*> ts) {
+  no_forward_gradient(op, ts);
   if (!at::GradMode::is_enabled()) return;
   for (const auto* t : ts)
     TORCH_CHECK(!t->defined() || !t->requires_grad(), op, " has no gradient: call it under torch.no_grad(), or on detached tensors");
@@ -700,7 +706,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_backward
     const at::Tensor& gq, const at::Tensor& gk, const at::Tensor& q, const at::Tensor& k, const OptTensor& qw,
     const OptTensor& kw, const at::Tensor& pos, const at::Tensor& rope, double eps, bool interleaved) {
   const at::Tensor none;
-  no_gradient("qk_norm_rope_backward", {&gq, &gk, &q, &k, given(qw) ? &*qw : &none, given(kw) ? &*kw : &none});
+  no_gradient("qk_norm_rope_backward", {&gq, &gk, &q, &k, given(qw) ? &*qw : &none, given(kw) ? &*kw : &none, &rope});
   at::AutoDispatchBelowADInplaceOrView below;
   static const auto op = c10::Dispatcher::singleton()
                              .findSchemaOrThrow("nnsx::qk_norm_rope_backward", "")

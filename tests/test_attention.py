@@ -267,6 +267,25 @@ def test_qk_norm_rope_part_of_the_gradient(ops):
         yk.sum().backward()
 
 
+def test_forward_mode_is_refused(ops):
+    """a tangent is not dropped unnoticed, under no_grad neither"""
+    import torch.autograd.forward_ad as fw
+
+    s = ref.batch([2, 1], [5, 9], 4, 2, 16, 4, torch.float32)
+    rope, pos, w, q, k = ops.rope_table(9, 16), torch.arange(3), torch.ones(16), s["q"], s["k"]
+    with fw.dual_level(), torch.no_grad():
+        def dual(x):
+            return fw.make_dual(x, torch.ones_like(x))
+
+        for a in ((dual(q), s["kc"], s["vc"]), (q, dual(s["kc"]), s["vc"]), (q, s["kc"], dual(s["vc"]))):
+            refused("no forward-mode gradient", ops.paged_attention, *a, s["table"], s["cu"], s["lens"])
+        for a in ((dual(q), k, s["v"], rope), (q, dual(k), s["v"], rope), (q, k, dual(s["v"]), rope), (q, k, s["v"], dual(rope))):
+            refused("no forward-mode gradient", ops.paged_append, *a[:3], s["kc"], s["vc"], s["table"], s["cu"], s["lens"], a[3])
+        for a in ((dual(q), k, w, rope), (q, k, dual(w), rope), (q, k, w, dual(rope))):
+            refused("no forward-mode gradient", ops.qk_norm_rope, a[0], a[1], a[2], None, pos, a[3])
+        refused("no forward-mode gradient", ops.qk_norm_rope_backward, dual(q), k, q, k, None, None, pos, rope)
+
+
 def test_append_is_seen_by_gradients(ops):
     """a cache that an earlier operation keeps for its gradient is not changed unnoticed"""
     s = ref.batch([2, 1], [5, 9], 4, 2, 16, 4, torch.float32)
