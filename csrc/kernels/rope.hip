@@ -167,15 +167,10 @@ __device__ __forceinline__ Lane<VEC> lane_of(int j, int d, int rot) {
 }
 
 // cosines and sines of this lane's pairs: cs[0] / sn[0] .. for half-split pieces
-// VEC pairs; interleaved pieces hold VEC / 2 pairs each.  Pairs that do not
-// turn get cos 1, sin 0.
+// VEC pairs; interleaved pieces hold VEC / 2 pairs each.  Of pieces that do not
+// turn: nothing.
 template <int VEC, bool INTER>
 __device__ __forceinline__ void load_angles(const float* row, const Lane<VEC>& l, int rot, float* cs, float* sn) {
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    cs[i] = 1.f;
-    sn[i] = 0.f;
-  }
   if (row == nullptr) return;
   if constexpr (INTER) {
 #pragma unroll
@@ -205,17 +200,22 @@ __device__ __forceinline__ void load_angles(const float* row, const Lane<VEC>& l
   }
 }
 
-// x[0 .. VEC) and x[VEC .. 2 VEC) turned by the angles (sign 1) or back (-1)
+// x[0 .. VEC) and x[VEC .. 2 VEC) turned by the angles (sign 1) or back (-1), where they turn at all: by an
+// angle of 0, an infinite value would make the one beside it NaN
 template <int VEC, bool INTER>
-__device__ __forceinline__ void turn(float* x, const float* cs, const float* sn, float sign) {
+__device__ __forceinline__ void turn(const Lane<VEC>& l, int rot, float* x, const float* cs, const float* sn, float sign) {
   if constexpr (INTER) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const float a = x[2 * i], b = x[2 * i + 1];
-      x[2 * i] = a * cs[i] - sign * b * sn[i];
-      x[2 * i + 1] = b * cs[i] + sign * a * sn[i];
-    }
-  } else {
+    for (int h = 0; h < 2; ++h)
+      if (l.c[h] < rot) {  // (a piece of 4 or 8 columns turns or does not: rot % 8 == 0)
+#pragma unroll
+        for (int i = h * VEC / 2; i < (h + 1) * VEC / 2; ++i) {
+          const float a = x[2 * i], b = x[2 * i + 1];
+          x[2 * i] = a * cs[i] - sign * b * sn[i];
+          x[2 * i + 1] = b * cs[i] + sign * a * sn[i];
+        }
+      }
+  } else if (l.turns) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       const float a = x[i], b = x[VEC + i];
@@ -353,7 +353,7 @@ __global__ __launch_bounds__(512) void rope_forward(RopeArgs a) {
 #pragma unroll
       for (int i = 0; i < 2 * VEC; ++i) x[i] *= inv * w[i];
     }
-    turn<VEC, INTER>(x, cs, sn, 1.f);
+    turn<VEC, INTER>(l, a.rot, x, cs, sn, 1.f);
   }
   E* yp;
   if (!APPEND || is_q) {
@@ -439,7 +439,7 @@ __global__ __launch_bounds__(512, 4) void rope_backward(RopeArgs a) {
         fetch();
       }
       if (there) {
-        turn<VEC, INTER>(g, cs, sn, -1.f);
+        turn<VEC, INTER>(l, a.rot, g, cs, sn, -1.f);
         float ss = 0.f, dot = 0.f;
 #pragma unroll
         for (int i = 0; i < 2 * VEC; ++i) ss += x[i] * x[i];

@@ -396,6 +396,46 @@ def test_paged_append(ops, dtype, inter, norm, rot, layout):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("dim,rot", [(24, 0), (24, 8), (64, 32), (128, 64), (128, 16), (72, 72)])
+def test_infinite_values_stay_in_their_columns(ops, dtype, inter, dim, rot):
+    """an infinite or NaN value reaches its own column and, within the rotated ones, the other of its pair"""
+    tokens = 40
+    gen = torch.Generator().manual_seed(dim + rot)
+    x = torch.randn(tokens, 3, dim, generator=gen).to(dtype)
+    for t in range(tokens):
+        x[t, t % 3, t * 7 % dim] = (float("inf"), float("-inf"), float("nan"))[t // 3 % 3]
+    x = x.cuda()
+    table, cu, lens = ints(*range(4))[None], ints(0, tokens), ints(tokens)
+    rope = ops.rope_table(tokens, rot).cuda() if rot else None
+    kc, vc = (torch.zeros(4, 3, 16, dim, device="cuda", dtype=dtype) for _ in range(2))
+    a = (table, cu, lens, rope, False, None, None, 1e-6, inter)
+    if not rot:  # nothing is turned: a copy
+        got = ops.paged_append(x, x, x, kc, vc, *a)
+        flat = [c[:, h].reshape(64, dim)[:tokens] for c in (kc, vc) for h in range(3)]
+        for y in (got, torch.stack(flat[:3], 1), torch.stack(flat[3:], 1)):
+            ref.close(y, x, torch.zeros(x.shape))
+        return
+    want = ref.append(x, x, x, kc, vc, *a)
+    got = ops.paged_append(x, x, x, kc, vc, *a)
+    for y, w in ((got, want[0]), (kc, want[1]), (vc, want[2])):
+        ref.close(y, *w)
+    # with the norm an infinite value makes its row zero but for its own column and pair; the weights' gradient likewise
+    g = torch.randn(tokens, 3, dim, generator=gen).to(dtype).cuda()
+    g[5, 1, dim - 1], g[6, 0, 0] = float("inf"), float("-inf")
+    x = x.nan_to_num(0.5, float("inf"), float("-inf"))
+    w, pos = torch.rand(dim, generator=gen).cuda() + 0.5, torch.arange(tokens, device="cuda")
+    for y in ops.qk_norm_rope(x, x, w, w, pos, rope, 1e-6, inter):
+        ref.close(y, *ref.norm_rope(x, w, pos, rope, 1e-6, inter))
+    clean = torch.randn(tokens, 3, dim, generator=gen).to(dtype).cuda()
+    d = ops.qk_norm_rope_backward(g, g, clean, clean, w, w, pos, rope, 1e-6, inter)
+    want = ref.norm_rope_grad(clean, w, g, pos, rope, 1e-6, inter)
+    for dx, dw in ((d[0], d[2]), (d[1], d[3])):
+        ref.close(dx, want[0], want[1])
+        ref.close(dw, want[2], want[3])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_paged_append_many_sequences(ops, dtype):
     new = [(i % 4) for i in range(300)]
     kv = [n + (i * 13) % 70 for i, n in enumerate(new)]
