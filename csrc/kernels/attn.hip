@@ -188,7 +188,8 @@ __device__ __forceinline__ Seq seq_of(const PagedAttnArgs& a, int b) {
   const int rows = s.n * a.group;  // (T * hq < 2^31)
   if (rows <= a.rows_lo || rows > a.rows_hi) s.n = 0;  // (the other form's)
   s.tiles = s.n > 0 ? static_cast<int>((static_cast<uint32_t>(rows) + ROWS - 1) / ROWS) : 0;
-  const int lo = a.window > 0 ? min(max(s.len - s.n - a.window + 1, 0), s.keys) : 0;
+  const int64_t first = static_cast<int64_t>(s.len) - s.n - a.window + 1;
+  const int lo = a.window > 0 ? static_cast<int>(min(max(first, static_cast<int64_t>(0)), static_cast<int64_t>(s.keys))) : 0;
   s.blocks = s.n > 0 ? static_cast<int>(static_cast<uint32_t>(s.keys + KEYS - 1) / KEYS - static_cast<uint32_t>(lo) / KEYS) : 0;
   return s;
 }

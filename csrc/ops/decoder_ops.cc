@@ -185,7 +185,7 @@ at::Tensor paged_attention_cuda(const at::Tensor& q0, const at::Tensor& k, const
   a.d = static_cast<int>(call.c.dim);
   a.scale = static_cast<float>(call.scale);
   a.causal = causal ? 1 : 0;
-  a.window = window < (1 << 30) ? static_cast<int>(window) : 0;  // (no position is farther)
+  a.window = static_cast<int>(std::min<int64_t>(window, std::numeric_limits<int>::max()));  // (no position is farther)
   at::Tensor ws;
   if (const size_t bytes = nnsx::kernels::paged_attn_workspace_bytes(a)) {
     ws = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));

@@ -214,6 +214,20 @@ def test_paged_attention_wide_window(ops, new):
         assert torch.equal(attend(ops, s, window=window), want), window
 
 
+@pytest.mark.parametrize("new", [1, 120])
+@pytest.mark.parametrize("window", [1, 2 ** 30 - 1, 2 ** 30, 2 ** 31 - 60, 2 ** 31 - 1, 2 ** 31, 2 ** 62])
+def test_paged_attention_window_behind_the_table(ops, window, new):
+    """lengths far behind the table: the window lies behind its keys, or reaches some or all of them"""
+    s = ref.batch([new, 1], [130, 77], 4, 1, 64, 16, torch.float32, "cuda", stale=0.0)
+    s["lens"] = ints(2 ** 31 - 1, 2 ** 31 - 40)
+    for causal in (True, False):
+        want = attend(ops, {n: t.cpu() for n, t in s.items()}, causal=causal, window=window)
+        assert bool((want == 0).all()) == (window <= 2 ** 30)
+        got = attend(ops, s, causal=causal, window=window)
+        # (fp32 twice: scores of 64 products, at most 144 weights; all values below 8)
+        assert (got.cpu() - want).abs().max() < 8 * (64 * 2 + 2 * 144 + 32) * 4 * ref.F32
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_paged_attention_strides(ops, dtype):
     """token-major cache memory, a table row wider than its tensor, queries cut from a fused projection"""
