@@ -38,7 +38,7 @@ struct PagedAttnArgs {
   int hq = 0, hkv = 0, d = 0;
   float scale = 1.f;
   int causal = 1;
-  int window = 0;       // 0: no window; else keys in (position - window, position]
+  int window = 0;       // 0: no window; else only keys from position - window + 1 on (up to the last, unless causal)
   void* ws = nullptr;   // paged_attn_workspace_bytes(a)
   // derived by the launcher: rows a token, and how the keys are split (attn.hip, plan)
   int group = 1, target = 0, min_chunk = 1, slots = 0, pairs = 0, parts = 0, apart = 1, one_round = 0, item_cost = 0, rows_lo = 0, rows_hi = 0;
