@@ -484,8 +484,10 @@ __host__ __device__ __forceinline__ size_t part_floats(int rows, int d) { return
 // O) are joined through LDS at the end.
 // Bound by the reads of the cache: 64 single tokens after 100 to 8192, 8 heads of 128 columns, bf16: 1.10 GB in
 // 222 us, 5.0 TB/s, as a large copy; two after 131072 and 120001, fp16: 1.03 GB in 186 us, 5.5 TB/s.  One after
-// 4096: 9.5 us, the plan and a few round trips to memory.  In fp32 a block of 128 columns is 128 matrix
-// instructions of 64 cycles, about as long as a wave's share of the reads takes, and a prompt is bound by them.
+// 4096: 9.5 us, the plan and a few round trips to memory.  In fp32 64 single tokens take 611 us (2.21 GB, 3.6 TB/s), and a
+// prompt of 2048 tokens, 32 heads of 128 columns, 477 us: 72 TFLOP/s of the pairs that count, a large product 153.
+// The matrix unit is busy for 46 % of that: a workgroup fills the registers of a SIMD's one wave, so that reads of K
+// and V (each again for every 32 rows), softmax and products mostly take turns.
 template <typename T>
 struct Elem { using type = uint16_t; static constexpr bool wide = false; };
 template <>
@@ -837,7 +839,8 @@ __global__ __launch_bounds__(kThreads, (DP <= 128 && !Elem<T>::wide) ? 2 : 1) vo
 // Bound by the matrix unit and what the waves issue beside it (a block of 128 columns: a softmax of 32
 // scores a lane, 48 LDS reads, the loads' addresses): 8192 tokens, 32 heads of 128 columns, bf16, causal: 540 to 570 us, 0.96 to 1.02
 // PFLOP/s of the pairs that count, where a large matrix product reaches 1.15; 4096 tokens, 16 heads of
-// 256 columns: 190 us, 0.72; 8192 tokens, 32 heads of 64 columns: 342 us, 0.80 (as many exponentials for half
+// 256 columns: 176 to 190 us, 0.72 to 0.78, the matrix unit busy for a third of the cycles: O, Q and the scores leave a
+// SIMD one wave, whose softmax runs beside nobody's products; 8192 tokens, 32 heads of 64 columns: 342 us, 0.80 (as many exponentials for half
 // the products).  Four pieces of V^T and six of K read ahead (two of V^T: 592 us, six: 582; four or eight of K: 578, 585).
 constexpr int kTileKeys = 64;
 
@@ -1407,6 +1410,10 @@ Plan plan_of(PagedAttnArgs a) {
   // Several: as many tokens as sequences (single tokens, as a rule), or no more rows than one tile has:
   // the stream form takes all (8 single tokens after 4096: 34, 40 by both; 2 x 16 tokens
   // after 8192: 33, 37).  Else both run, each on its own sequences (8 x 16 tokens after 4096: 58, stream form 71).
+  // Single tokens with rows of padding behind them run both, with fewer splits (64 tokens after 2048: 107 without padding,
+  // 124 with 1 to 64 rows of it; 64 after 100 to 8192: 224 and 253; 8 after 4096: 38 either way), and a chunk among as
+  // many tokens as slots takes the stream form (200 tokens after 4096, 56 single ones, 199 empty slots: 122; 119
+  // by both, with one row more).
   if (a.type == AttnType::kF32)
     p.tile = false;
   else if (a.p.B == 1)
