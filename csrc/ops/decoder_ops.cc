@@ -748,6 +748,9 @@ at::Tensor paged_append_inplace(const OptTensor& q, const at::Tensor& k, const a
                                 at::Tensor& v_cache, const at::Tensor& table, const at::Tensor& cu, const at::Tensor& len,
                                 const OptTensor& rope, bool norm, const OptTensor& qw, const OptTensor& kw, double eps,
                                 bool interleaved) {
+  for (const auto* t : {&k_cache, &v_cache})  // (the count of changes below would refuse it, after the change)
+    TORCH_CHECK(!t->is_inference() || c10::InferenceMode::is_enabled(),
+                "paged_append: a cache made in inference mode can be changed in inference mode only");
   at::Tensor out;
   {
     at::AutoDispatchBelowADInplaceOrView below;

@@ -267,6 +267,21 @@ def test_qk_norm_rope_part_of_the_gradient(ops):
         yk.sum().backward()
 
 
+def test_append_to_a_cache_of_inference_mode(ops):
+    """outside that mode it is refused before a row is written"""
+    s = ref.batch([2, 1], [5, 9], 4, 2, 16, 4, torch.float32, stale=0.0)
+    with torch.inference_mode():
+        kc, vc = s["kc"].clone(), s["vc"].clone()
+    a = (s["k"], s["v"]), (s["table"], s["cu"], s["lens"])
+    for k, v in ((kc, s["vc"]), (s["kc"], vc)):
+        before = k.clone(), v.clone()
+        refused("inference mode", ops.paged_append, None, *a[0], k, v, *a[1])
+        assert torch.equal(k, before[0]) and torch.equal(v, before[1])
+    with torch.inference_mode():
+        ops.paged_append(None, *a[0], kc, vc, *a[1])
+        assert not torch.equal(kc, s["kc"])
+
+
 def test_forward_mode_is_refused(ops):
     """a tangent is not dropped unnoticed, under no_grad neither"""
     import torch.autograd.forward_ad as fw
