@@ -1222,7 +1222,7 @@ __global__ __launch_bounds__(kTileWaves<DP> * 64, DP <= 64 ? 3 : 2) void paged_a
 // groups divide the live rows and, where there are few, a row's splits, whose
 // parts are added through LDS in a fixed order.  A pair's rows are dealt out to
 // a.apart workgroups: few pairs are spread over more of the card.  4 to 7 us, a launch, the plan and a round
-// trip; 15 us for the tiles of that mixed batch.
+// trip; 13 us for the tiles of that mixed batch.
 constexpr int kJoinThreads = 256;
 
 template <typename T, int ROWS, int KEYS, int LG>
